@@ -270,6 +270,36 @@ int sjh_add_ln(float* X, const void* R, const float* W, const float* B, void* Y,
                int32_t D, float eps, int32_t residual, int32_t bias, int32_t dtype,
                sjh_stream_t stream);
 
+/* The norms on both sides of a block fused with its gate and residual scales:
+ *   u  = post(r)                                 (r: the block's output)
+ *   x' = x_scale * x + r_scale * gate[row] * u   (fp32 residual stream)
+ *   y  = pre(x')                                 (the next block's input)
+ * post and pre are nothing, LayerNorm ((v - mean) / sqrt(var + eps) * w + b,
+ * population variance) or the RMS norm (v / sqrt(mean(v^2) + eps) * w + b).
+ * sjh_add_ln is post = nothing, pre = LayerNorm, without gate or scales.  No
+ * counterpart in the reference, whose blocks have no norm after them.
+ * D up to 8192.  Row strides are in elements, 0 standing for D; rows whose
+ * strides and addresses allow 16-byte accesses (8-byte for bf16) of four
+ * values are the fast ones.  x_out may be x, and y may be r, with the same
+ * strides; no other outputs and inputs may overlap.  Sums are taken in double.
+ * A NaN in r or x, or an infinity under LayerNorm, reaches its own row only. */
+enum { SJH_NORM_NONE = 0, SJH_NORM_LAYER = 1, SJH_NORM_RMS = 2 };
+typedef struct sjh_add_norm_args {
+  const float* x;          /* [M, D] */
+  const void* r;           /* [M, D] of dtype, or NULL: u = 0 */
+  float* x_out;            /* [M, D], or NULL: x' is not stored */
+  void* y;                 /* [M, D] of dtype, or NULL: only x' */
+  const float *post_w, *post_b; /* [D], each NULL: 1, 0 */
+  const float *pre_w, *pre_b;   /* [D], each NULL: 1, 0 */
+  const float* gate;       /* [n_gates, D], or NULL: 1 */
+  const int32_t* gate_row; /* [M] gate row of each row, clamped to [0, n_gates), or NULL: row 0 */
+  int64_t ld_x, ld_r, ld_xo, ld_y;
+  float x_scale, r_scale, eps;
+  int32_t post_norm, pre_norm; /* SJH_NORM_* */
+  int32_t n_gates, M, D, dtype;
+} sjh_add_norm_args;
+int sjh_add_norm(const sjh_add_norm_args* args, sjh_stream_t stream);
+
 /* sj_rope (cuda/kernels.cu:282-288): in-place rotate-half on packed qkv
  * [M, 3*H*Dh], row r at position r % L; cos/sin fp32 [L_max, Dh/2]. */
 int sjh_rope(void* qkv, const float* cos_t, const float* sin_t, int64_t M, int32_t L, int32_t H,

@@ -60,6 +60,18 @@ class Options(C.Structure):
                 ("fuse_attn_wo", C.c_int32)]
 
 
+SJH_NORM_NONE, SJH_NORM_LAYER, SJH_NORM_RMS = 0, 1, 2
+
+
+class AddNormArgs(C.Structure):
+    """sjh_add_norm_args: pointers as integers (tensor.data_ptr()) or None."""
+    _fields_ = [*[(n, C.c_void_p) for n in ("x", "r", "x_out", "y", "post_w", "post_b", "pre_w", "pre_b", "gate",
+                                            "gate_row")],
+                *[(n, C.c_int64) for n in ("ld_x", "ld_r", "ld_xo", "ld_y")],
+                *[(n, C.c_float) for n in ("x_scale", "r_scale", "eps")],
+                *[(n, C.c_int32) for n in ("post_norm", "pre_norm", "n_gates", "M", "D", "dtype")]]
+
+
 # Every symbol include/snapjudge_hip.h declares, with its ctypes signature.
 _SIGS = {
     "sjh_last_error": (C.c_char_p, []),
@@ -97,6 +109,7 @@ _SIGS = {
     "sjh_add_ln": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                              C.c_int32, C.c_int32, C.c_float, C.c_int32, C.c_int32, C.c_int32,
                              C.c_void_p]),
+    "sjh_add_norm": (C.c_int, [C.POINTER(AddNormArgs), C.c_void_p]),
     "sjh_rope": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_int32,
                            C.c_int32, C.c_int32, C.c_void_p]),
     "sjh_attn": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32,

@@ -56,6 +56,17 @@ hipStream_t as_stream(sjh_stream_t s) { return reinterpret_cast<hipStream_t>(s);
 
 size_t esize(int32_t dt) { return dt == SJH_BF16 ? 2 : 4; }
 
+// The stream of a call must be one of the current device, whose memory the
+// pointers are taken to be in.
+void check_stream(sjh_stream_t s) {
+  if (!s) return;
+  int cur = 0;
+  hipDevice_t dev = 0;
+  sjh::hip_check(hipGetDevice(&cur), "hipGetDevice");
+  sjh::hip_check(hipStreamGetDevice(as_stream(s), &dev), "hipStreamGetDevice");
+  if (dev != cur) sjh::fail_arg("the stream belongs to another device than the current one");
+}
+
 void check_dtype(int32_t dt) {
   if (dt != SJH_F32 && dt != SJH_BF16) sjh::fail("dtype must be SJH_F32 or SJH_BF16");
 }
@@ -369,6 +380,38 @@ int sjh_add_ln(float* X, const void* R, const float* W, const float* B, void* Y,
     a.M = M;
     a.D = D;
     sjh::launch_ln(a, as_stream(stream));
+  });
+}
+
+int sjh_add_norm(const sjh_add_norm_args* p, sjh_stream_t stream) {
+  return guarded([&] {
+    if (!p) sjh::fail_arg("add_norm: null arguments");
+    sjh::AddNormArgs a;
+    a.x = p->x;
+    a.r = p->r;
+    a.x_out = p->x_out;
+    a.y = p->y;
+    a.post_w = p->post_w;
+    a.post_b = p->post_b;
+    a.pre_w = p->pre_w;
+    a.pre_b = p->pre_b;
+    a.gate = p->gate;
+    a.gate_row = p->gate_row;
+    a.ld_x = p->ld_x ? p->ld_x : p->D;
+    a.ld_r = p->ld_r ? p->ld_r : p->D;
+    a.ld_xo = p->ld_xo ? p->ld_xo : p->D;
+    a.ld_y = p->ld_y ? p->ld_y : p->D;
+    a.x_scale = p->x_scale;
+    a.r_scale = p->r_scale;
+    a.eps = p->eps;
+    a.post_norm = p->post_norm;
+    a.pre_norm = p->pre_norm;
+    a.n_gates = p->n_gates;
+    a.M = p->M;
+    a.D = p->D;
+    a.dtype = p->dtype;
+    if (a.M > 0) check_stream(stream);
+    sjh::launch_add_norm(a, as_stream(stream));
   });
 }
 

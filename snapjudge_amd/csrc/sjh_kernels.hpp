@@ -198,6 +198,23 @@ void launch_ln(const LnArgs& a, hipStream_t st);
 // D <= 1024 with 16-byte aligned fp32 rows.
 bool ln_takes_parts(const LnArgs& a);
 
+// sjh_add_norm's arguments (include/snapjudge_hip.h), strides filled in.
+enum NormKind : int { NORM_NONE = 0, NORM_LAYER = 1, NORM_RMS = 2 };
+struct AddNormArgs {
+  const float* x = nullptr;
+  const void* r = nullptr;
+  float* x_out = nullptr;
+  void* y = nullptr;
+  const float *post_w = nullptr, *post_b = nullptr, *pre_w = nullptr, *pre_b = nullptr;
+  const float* gate = nullptr;
+  const int* gate_row = nullptr;
+  int64_t ld_x = 0, ld_r = 0, ld_xo = 0, ld_y = 0;
+  float x_scale = 1.f, r_scale = 1.f, eps = 1e-5f;
+  int post_norm = NORM_NONE, pre_norm = NORM_NONE;
+  int n_gates = 0, M = 0, D = 0, dtype = DT_BF16;
+};
+void launch_add_norm(const AddNormArgs& a, hipStream_t st);
+
 // Non-causal attention over a varlen batch.  Sequence b owns rows
 // [seq_start[b], seq_start[b] + max(q_len[b], k_len[b])); its queries are the
 // first q_len[b] rows and its keys/values the first k_len[b] rows.  Head h of

@@ -86,3 +86,19 @@ def test_model_create_without_gpu_fails_cleanly():
     with pytest.raises(sj.SjhError) as e:
         sj.Model(w, synth.flat_cfg(rl, enc))
     assert e.value.code in (-1, -2)
+
+
+def refused(fn, args, text):
+    rc = fn(C.byref(args), None)
+    assert rc == -1 and text in sj.lib().sjh_last_error(), (rc, sj.lib().sjh_last_error())
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(M=-1), b"M must not"), (dict(D=0), b"D must"), (dict(D=8193), b"D must"), (dict(dtype=2), b"dtype"), (dict(post_norm=3), b"unknown norm"),
+    (dict(pre_norm=-1), b"unknown norm"), (dict(ld_x=15), b"stride"), (dict(ld_y=-3), b"stride"), (dict(eps=-1.0), b"eps"),
+    (dict(eps=float("nan")), b"eps"), (dict(gate=16), b"n_gates"), (dict(gate_row=16), b"without gates"), (dict(x=None), b"null x"),
+    (dict(x_out=None), b"neither")])
+def test_add_norm_refuses(change, text):
+    kw = dict(x=16, x_out=16, x_scale=1.0, r_scale=1.0, eps=1e-5, M=4, D=16, dtype=sj.SJH_F32)
+    refused(sj.lib().sjh_add_norm, sj.AddNormArgs(**{**kw, **change}), text)
+    assert sj.lib().sjh_add_norm(None, None) == -1
