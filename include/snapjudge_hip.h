@@ -319,6 +319,58 @@ int sjh_attn(const void* qkv, const int32_t* lens, void* O, int32_t B, int32_t L
 int sjh_attn_log2(const void* qkv, const int32_t* lens, void* O, int32_t B, int32_t L, int32_t H,
                   int32_t window, sjh_stream_t stream);
 
+/* Attention with modified scores over a varlen batch, with as many key heads
+ * as there are or fewer, for full sequences, chunks of them or single tokens:
+ *   s(p, j) = softcap * tanh(scale q_p.k_j / softcap) - slopes[h] |p - j|
+ *   o_p     = sum over the visible keys j of softmax_j(s(p, .)) v_j
+ * Key j (its index in the sequence's keys) is visible to the query at position
+ * p = q_pos + (its index in the sequence's queries) where
+ *   j < prefix, or
+ *   (not causal, or j <= p) and (window 0, or |p - j| <= window) and
+ *   (no documents, or q_doc of the query's row == k_doc of the key's row).
+ * A query that sees no key gives zeros.  A key takes part only where it is
+ * visible, whatever its values (infinities and NaN among them).  sjh_attn is
+ * the padded, unmodified case; no counterpart in the reference, whose masks
+ * are padding and a window (src/tensor.cpp:186-192).
+ *
+ * Sequence b's queries are rows q_start[b] + [0, q_len[b]) of q and o, its keys
+ * rows k_start[b] + [0, k_len[b]) of k and v; head h of row t is at
+ * q + t ld_q + h Dh (k, v: head h / (H / Hkv)).  Rows of o outside every
+ * sequence are left as they were.  Starts and lengths are clamped to q_rows,
+ * k_rows, max_q and max_k (so max_q and max_k must bound the lengths), q_pos to
+ * [0, 2^29], prefix to [0, k_len].  Dh 8, 16, 32, 64 or 128; bf16 with Dh 64 or
+ * 128, row strides a multiple of 8 (o: 4) and 16-byte (o: 8-byte) aligned
+ * tensors runs on the bf16 matrix pipes, all else in fp32 products.
+ *
+ * workspace: sjh_attn_scored_workspace bytes (often 0), 16-byte aligned, free
+ * again once the call's work is done; calls that may overlap (streams, graphs)
+ * need one each.  It depends on B, H, Hkv, Dh, max_q, max_k, window, dtype and
+ * the strides and addresses of the tensors. */
+typedef struct sjh_attn_scored_args {
+  const void *q, *k, *v; /* rows of dtype */
+  void* o;
+  const int32_t *q_start, *q_len; /* [B] */
+  const int32_t *k_start, *k_len; /* [B], or both NULL: q_start, q_len */
+  const int32_t* q_pos;  /* [B] position of each sequence's first query, or NULL: 0 */
+  const int32_t* prefix; /* [B], or NULL: 0 */
+  const int32_t *q_doc, *k_doc; /* [q_rows], [k_rows] document of each row, or both NULL */
+  const float* slopes;   /* [H] finite, or NULL: 0 */
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t ld_q, ld_k, ld_v, ld_o; /* row strides in elements, 0: H Dh (k, v: Hkv Dh) */
+  float scale;    /* > 0, or 0: 1 / sqrt(Dh) */
+  float softcap;  /* > 0, or 0: no cap */
+  int32_t window; /* >= 0 */
+  int32_t causal;
+  int32_t B, H, Hkv, Dh; /* Hkv divides H; 0: H */
+  int32_t q_rows, k_rows; /* rows of q and o, of k and v; at most 2^29 */
+  int32_t max_q, max_k;   /* upper bounds of the lengths */
+  int32_t dtype;
+} sjh_attn_scored_args;
+/* Bytes of workspace that a call of these arguments needs, or SJH_E_INVALID. */
+int64_t sjh_attn_scored_workspace(const sjh_attn_scored_args* args);
+int sjh_attn_scored(const sjh_attn_scored_args* args, sjh_stream_t stream);
+
 /* Embedding gather + LayerNorm (src/model.cpp:332-340): X[r] = LN(table[ids[r]]) * w.
  * table [V, D] of dtype, ids int32 [M], X fp32 [M, D]. */
 int sjh_embed_ln(const void* table, const int32_t* ids, const float* w, float* X, int32_t M,

@@ -72,6 +72,16 @@ class AddNormArgs(C.Structure):
                 *[(n, C.c_int32) for n in ("post_norm", "pre_norm", "n_gates", "M", "D", "dtype")]]
 
 
+class AttnScoredArgs(C.Structure):
+    """sjh_attn_scored_args: pointers as integers (tensor.data_ptr()) or None."""
+    _fields_ = [*[(n, C.c_void_p) for n in ("q", "k", "v", "o", "q_start", "q_len", "k_start", "k_len", "q_pos", "prefix",
+                                            "q_doc", "k_doc", "slopes", "workspace")],
+                *[(n, C.c_int64) for n in ("workspace_bytes", "ld_q", "ld_k", "ld_v", "ld_o")],
+                ("scale", C.c_float), ("softcap", C.c_float),
+                *[(n, C.c_int32) for n in ("window", "causal", "B", "H", "Hkv", "Dh", "q_rows", "k_rows", "max_q", "max_k",
+                                           "dtype")]]
+
+
 # Every symbol include/snapjudge_hip.h declares, with its ctypes signature.
 _SIGS = {
     "sjh_last_error": (C.c_char_p, []),
@@ -116,6 +126,8 @@ _SIGS = {
                            C.c_int32, C.c_int32, C.c_int32, C.c_void_p]),
     "sjh_attn_log2": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32,
                                 C.c_int32, C.c_void_p]),
+    "sjh_attn_scored_workspace": (C.c_int64, [C.POINTER(AttnScoredArgs)]),
+    "sjh_attn_scored": (C.c_int, [C.POINTER(AttnScoredArgs), C.c_void_p]),
     "sjh_embed_ln": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32,
                                C.c_int32, C.c_float, C.c_int32, C.c_void_p]),
 }

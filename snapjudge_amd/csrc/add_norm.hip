@@ -29,6 +29,7 @@ namespace {
 constexpr int kWpb = 4;          // waves per workgroup of the batch kernels
 constexpr int kWaveMaxD = 1024;  // columns of a row that one wave holds
 constexpr int kMaxD = 8192;      // ... that a workgroup of four holds
+constexpr unsigned kGridX = 1u << 22;  // workgroups of a grid's row: a grid dimension holds fewer than 2^32 threads
 
 // V consecutive values of a row, V = 4 (vector accesses) or 1.
 template <int V, typename T>
@@ -96,8 +97,9 @@ __global__ __launch_bounds__(64 * WPB) void add_norm_kernel(AddNormArgs a) {
   constexpr int TPR = 64 * WAVES;  // threads per row
   __shared__ double red[2][2 * WPB];
   const int t = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;
-  const int row = __builtin_amdgcn_readfirstlane(WAVES == 1 ? blockIdx.x * WPB + (threadIdx.x >> 6) : blockIdx.x);
-  if (row >= a.M) return;  // uniform over the wave (WAVES 1) or the workgroup
+  const unsigned wg = blockIdx.y * kGridX + blockIdx.x;
+  const int64_t row = __builtin_amdgcn_readfirstlane(WAVES == 1 ? wg * WPB + (threadIdx.x >> 6) : wg);
+  if (static_cast<unsigned>(row) >= static_cast<unsigned>(a.M)) return;  // uniform over the wave (WAVES 1) or the workgroup
   const int D = a.D, np = D / V;
   float x[NV][V], u[NV][V], g[NV][V], pw[NV][V], pb[NV][V], w[NV][V], b[NV][V];
   const float* gate = nullptr;
@@ -105,10 +107,10 @@ __global__ __launch_bounds__(64 * WPB) void add_norm_kernel(AddNormArgs a) {
     const int id = a.gate_row ? min(max(a.gate_row[row], 0), a.n_gates - 1) : 0;
     gate = a.gate + static_cast<int64_t>(id) * D;
   }
-  const float* xr = a.x + static_cast<int64_t>(row) * a.ld_x;
+  const float* xr = a.x + row * a.ld_x;
   // (read before x_out, which may be x, is written)
   const float first_x = WAVES == 1 ? 0.f : xr[0];
-  const T* rr = a.r ? static_cast<const T*>(a.r) + static_cast<int64_t>(row) * a.ld_r : nullptr;
+  const T* rr = a.r ? static_cast<const T*>(a.r) + row * a.ld_r : nullptr;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = t + TPR * i;
@@ -138,7 +140,7 @@ __global__ __launch_bounds__(64 * WPB) void add_norm_kernel(AddNormArgs a) {
       for (int k = 0; k < V; ++k) x[i][k] *= a.x_scale;
   }
   if (a.x_out) {
-    float* xo = a.x_out + static_cast<int64_t>(row) * a.ld_xo;
+    float* xo = a.x_out + row * a.ld_xo;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if (t + TPR * i < np) storev<V>(xo + V * (t + TPR * i), x[i]);
@@ -150,24 +152,29 @@ __global__ __launch_bounds__(64 * WPB) void add_norm_kernel(AddNormArgs a) {
                                 : a.x_scale * first_x;
     norm_row<NV, V, WAVES>(x, w, b, a.pre_norm, x0, t, np, D, a.eps, red[1]);
   }
-  T* yo = static_cast<T*>(a.y) + static_cast<int64_t>(row) * a.ld_y;
+  T* yo = static_cast<T*>(a.y) + row * a.ld_y;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
     if (t + TPR * i < np) storev<V>(yo + V * (t + TPR * i), x[i]);
+}
+
+dim3 grid_of(int wgs) {
+  const unsigned n = static_cast<unsigned>(wgs);
+  return dim3(n < kGridX ? n : kGridX, (n + kGridX - 1) / kGridX);
 }
 
 template <int NV, int V, typename T>
 void launch_wave_rows(const AddNormArgs& a, hipStream_t st) {
   // one row per workgroup while that leaves CUs without a row, four beyond
   if (a.M <= 2 * num_cus())
-    add_norm_kernel<NV, V, 1, 1, T><<<a.M, 64, 0, st>>>(a);
+    add_norm_kernel<NV, V, 1, 1, T><<<grid_of(a.M), 64, 0, st>>>(a);
   else
-    add_norm_kernel<NV, V, 1, kWpb, T><<<(a.M + kWpb - 1) / kWpb, 64 * kWpb, 0, st>>>(a);
+    add_norm_kernel<NV, V, 1, kWpb, T><<<grid_of(a.M / kWpb + (a.M % kWpb != 0)), 64 * kWpb, 0, st>>>(a);
 }
 
 template <int NV, int V, typename T>
 void launch_group_rows(const AddNormArgs& a, hipStream_t st) {
-  add_norm_kernel<NV, V, kWpb, kWpb, T><<<a.M, 64 * kWpb, 0, st>>>(a);
+  add_norm_kernel<NV, V, kWpb, kWpb, T><<<grid_of(a.M), 64 * kWpb, 0, st>>>(a);
 }
 
 template <typename T>

@@ -67,6 +67,64 @@ void check_stream(sjh_stream_t s) {
   if (dev != cur) sjh::fail_arg("the stream belongs to another device than the current one");
 }
 
+// sjh_attn_scored's arguments, checked (but for the pointers) and completed.
+sjh::AttnScoredArgs scored_args(const sjh_attn_scored_args* p) {
+  using sjh::fail_arg;
+  if (!p) fail_arg("attn_scored: null arguments");
+  constexpr int32_t kMaxRows = 1 << 29;
+  if (p->dtype != SJH_F32 && p->dtype != SJH_BF16) fail_arg("attn_scored: dtype must be SJH_F32 or SJH_BF16");
+  if (p->B < 0 || p->H < 1 || p->Hkv < 0) fail_arg("attn_scored: bad batch or heads");
+  const int32_t hkv = p->Hkv ? p->Hkv : p->H;
+  if (p->H % hkv != 0) fail_arg("attn_scored: Hkv must divide H");
+  if (p->Dh != 8 && p->Dh != 16 && p->Dh != 32 && p->Dh != 64 && p->Dh != 128)
+    fail_arg("attn_scored: head_dim must be 8, 16, 32, 64 or 128");
+  if (p->q_rows < 0 || p->k_rows < 0 || p->q_rows > kMaxRows || p->k_rows > kMaxRows)
+    fail_arg("attn_scored: q_rows and k_rows must lie in [0, 2^29]");
+  if (p->max_q < 0 || p->max_k < 0) fail_arg("attn_scored: negative length bound");
+  if (!(p->scale >= 0.f) || !(p->scale < INFINITY)) fail_arg("attn_scored: scale must be finite and not negative");
+  if (!(p->softcap >= 0.f) || !(p->softcap < INFINITY)) fail_arg("attn_scored: softcap must be finite and not negative");
+  if (p->window < 0) fail_arg("attn_scored: negative window");
+  if (!p->q_doc != !p->k_doc) fail_arg("attn_scored: documents of queries and keys, or of neither");
+  if (!p->k_start != !p->k_len) fail_arg("attn_scored: k_start and k_len, or neither");
+  sjh::AttnScoredArgs a;
+  a.q = p->q;
+  a.k = p->k;
+  a.v = p->v;
+  a.o = p->o;
+  const int64_t qd = static_cast<int64_t>(p->H) * p->Dh, kd = static_cast<int64_t>(hkv) * p->Dh;
+  a.ld_q = p->ld_q ? p->ld_q : qd;
+  a.ld_k = p->ld_k ? p->ld_k : kd;
+  a.ld_v = p->ld_v ? p->ld_v : kd;
+  a.ld_o = p->ld_o ? p->ld_o : qd;
+  if (a.ld_q < qd || a.ld_o < qd || a.ld_k < kd || a.ld_v < kd) fail_arg("attn_scored: row stride < heads * Dh");
+  // (a tile's rows are addressed by 32-bit byte offsets)
+  if (a.ld_k > (1 << 23) || a.ld_v > (1 << 23)) fail_arg("attn_scored: key row stride above 2^23");
+  a.q_start = p->q_start;
+  a.q_len = p->q_len;
+  a.k_start = p->k_start ? p->k_start : p->q_start;
+  a.k_len = p->k_len ? p->k_len : p->q_len;
+  a.q_pos = p->q_pos;
+  a.prefix = p->prefix;
+  a.q_doc = p->q_doc;
+  a.k_doc = p->k_doc;
+  a.slopes = p->slopes;
+  a.scale = p->scale > 0.f ? p->scale : 1.0f / std::sqrt(static_cast<float>(p->Dh));
+  a.softcap = p->softcap;
+  // positions differ by less than 2^30: a wider window hides nothing
+  a.window = p->window < (1 << 30) - 2 ? p->window : 0;
+  a.causal = p->causal != 0;
+  a.B = p->B;
+  a.H = p->H;
+  a.Hkv = hkv;
+  a.Dh = p->Dh;
+  a.q_rows = p->q_rows;
+  a.k_rows = p->k_rows;
+  a.max_q = p->max_q < p->q_rows ? p->max_q : p->q_rows;
+  a.max_k = p->max_k < p->k_rows ? p->max_k : p->k_rows;
+  a.dtype = p->dtype;
+  return a;
+}
+
 void check_dtype(int32_t dt) {
   if (dt != SJH_F32 && dt != SJH_BF16) sjh::fail("dtype must be SJH_F32 or SJH_BF16");
 }
@@ -475,6 +533,32 @@ int sjh_attn_log2(const void* qkv, const int32_t* lens, void* O, int32_t B, int3
     a.scale = 0.125f;
     a.q_log2_scaled = true;
     sjh::launch_attn(a, as_stream(stream));
+  });
+}
+
+int64_t sjh_attn_scored_workspace(const sjh_attn_scored_args* p) {
+  int64_t n = 0;
+  const int rc = guarded([&] {
+    const sjh::AttnScoredArgs a = scored_args(p);
+    if (a.B > 0 && a.max_q > 0) n = sjh::attn_scored_part_bytes(a);
+  });
+  return rc == SJH_OK ? n : rc;
+}
+
+int sjh_attn_scored(const sjh_attn_scored_args* p, sjh_stream_t stream) {
+  return guarded([&] {
+    sjh::AttnScoredArgs a = scored_args(p);
+    if (a.B == 0 || a.max_q == 0) return;
+    if (!a.q || !a.o || !a.q_start || !a.q_len || (a.max_k > 0 && (!a.k || !a.v)))
+      sjh::fail_arg("attn_scored: null pointer");
+    const int64_t need = sjh::attn_scored_part_bytes(a);
+    if (need > 0) {
+      if (!p->workspace || p->workspace_bytes < need) sjh::fail_arg("attn_scored: workspace too small");
+      if (reinterpret_cast<uintptr_t>(p->workspace) & 15u) sjh::fail_arg("attn_scored: workspace must be 16-byte aligned");
+      a.part = static_cast<float*>(p->workspace);
+    }
+    check_stream(stream);
+    sjh::launch_attn_scored(a, as_stream(stream));
   });
 }
 

@@ -271,6 +271,37 @@ struct AttnArgs {
 constexpr int kAttnWoCols = 128;
 void launch_attn(const AttnArgs& a, hipStream_t st);
 
+// sjh_attn_scored's arguments (include/snapjudge_hip.h), strides and scale
+// filled in.  Sequence b's queries are rows [q_start[b], + q_len[b]) of q and
+// o, its keys rows [k_start[b], + k_len[b]) of k and v; the kernels clamp both
+// to the rows that there are (q_rows, k_rows) and to max_q and max_k.
+struct AttnScoredArgs {
+  const void *q = nullptr, *k = nullptr, *v = nullptr;
+  void* o = nullptr;
+  int64_t ld_q = 0, ld_k = 0, ld_v = 0, ld_o = 0;
+  const int *q_start = nullptr, *q_len = nullptr, *k_start = nullptr, *k_len = nullptr;
+  const int* q_pos = nullptr;   // position of a sequence's first query, or null: 0
+  const int* prefix = nullptr;  // keys that every query of a sequence sees, or null: 0
+  const int *q_doc = nullptr, *k_doc = nullptr;  // document of each row, or null
+  const float* slopes = nullptr;                 // [H] or null
+  float scale = 0.f, softcap = 0.f;
+  int window = 0, causal = 0;
+  int B = 0, H = 0, Hkv = 0, Dh = 0;
+  int q_rows = 0, k_rows = 0, max_q = 0, max_k = 0;
+  int dtype = DT_BF16;
+  float* part = nullptr;  // partial results of split items (workspace)
+  // set by the launcher: query blocks per head (or group of heads), queries
+  // per block and splits
+  int n_blocks = 0, splits = 1;
+  int pack = 0;  // a block holds the max_q queries of every head of its group
+};
+// Bytes of AttnScoredArgs::part that a launch needs (0: none).  Depends on the
+// sizes and the type alone.
+int64_t attn_scored_part_bytes(const AttnScoredArgs& a);
+void launch_attn_scored(const AttnScoredArgs& a, hipStream_t st);
+// launch_attn_scored's fp32-product kernel (checked arguments).
+void launch_attn_scored_f32(const AttnScoredArgs& a, hipStream_t st);
+
 // Attention work list of a batch (AttnArgs::items): the (sequence, head,
 // query block of kAttnQ rows) items of the sequences in table order (longest
 // first), each sequence's heads in turn and each head's blocks in turn, are

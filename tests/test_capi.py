@@ -102,3 +102,28 @@ def test_add_norm_refuses(change, text):
     kw = dict(x=16, x_out=16, x_scale=1.0, r_scale=1.0, eps=1e-5, M=4, D=16, dtype=sj.SJH_F32)
     refused(sj.lib().sjh_add_norm, sj.AddNormArgs(**{**kw, **change}), text)
     assert sj.lib().sjh_add_norm(None, None) == -1
+
+
+SCORED = dict(q=16, k=16, v=16, o=16, q_start=16, q_len=16, B=1, H=4, Hkv=2, Dh=64, q_rows=8, k_rows=8, max_q=8, max_k=8, dtype=sj.SJH_BF16)
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(dtype=2), b"dtype"), (dict(B=-1), b"batch or heads"), (dict(H=0), b"batch or heads"), (dict(Hkv=3), b"divide"), (dict(Dh=24), b"head_dim"),
+    (dict(q_rows=-1), b"q_rows"), (dict(k_rows=(1 << 29) + 1), b"k_rows"), (dict(max_q=-1), b"length bound"), (dict(scale=-1.0), b"scale"),
+    (dict(scale=float("nan")), b"scale"), (dict(softcap=float("inf")), b"softcap"), (dict(softcap=-2.0), b"softcap"), (dict(window=-1), b"window"),
+    (dict(q_doc=16), b"documents"), (dict(k_doc=16), b"documents"), (dict(k_len=16), b"k_start"), (dict(ld_q=255), b"stride"), (dict(ld_v=64), b"stride"),
+    (dict(ld_k=(1 << 23) + 8), b"2^23"), (dict(o=None), b"null"), (dict(k=None), b"null"), (dict(q_len=None), b"null"),
+    (dict(k_rows=9000, max_k=9000), b"workspace too small"), (dict(k_rows=9000, max_k=9000, workspace=24, workspace_bytes=1 << 30), b"aligned"),
+    (dict(B=1 << 22, q_rows=1 << 20, max_q=1 << 20, H=16, Hkv=16), b"too many")])
+def test_attn_scored_refuses(change, text):
+    refused(sj.lib().sjh_attn_scored, sj.AttnScoredArgs(**{**SCORED, **change}), text)
+    assert sj.lib().sjh_attn_scored(None, None) == -1
+
+
+def test_attn_scored_workspace_is_a_function_of_the_sizes():
+    ws = lambda **kw: sj.lib().sjh_attn_scored_workspace(C.byref(sj.AttnScoredArgs(**{**SCORED, **kw})))  # noqa: E731
+    assert ws() == 0  # one short sequence: nothing to split
+    assert ws(k_rows=9000, max_k=9000) > 0
+    assert ws(k_rows=9000, max_k=9000, window=50) == 0
+    assert ws(k_rows=9000, max_k=9000, B=0) == 0
+    assert ws(Dh=7) == -1 and b"head_dim" in sj.lib().sjh_last_error()
