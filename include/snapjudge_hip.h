@@ -245,6 +245,39 @@ int sjh_quantize_fp8(const float* w, int64_t rows, int64_t cols, uint8_t* q, flo
 int sjh_gemm_fp8w(const void* A, const uint8_t* Wq, const float* w_scale, const float* bias,
                   void* C, int32_t M, int32_t N, int32_t K, int32_t act, sjh_stream_t stream);
 
+/* Low-rank adapters of many requests beside a shared projection:
+ *   out[m] = act(x[m] . W^T + bias + scale[a] (x[m] . A_a^T) . B_a^T), a = adapter[m]
+ * A row whose adapter lies outside [0, n_adapters) has none: its values are
+ * sjh_gemm's (sjh_gemm_fp8w's).  Rows of any adapters in any order; no row's
+ * values depend on another row's adapter, infinities and NaN included.  Ranks
+ * below R: zero rows of B_a.  The reference's model has one adapter, behind
+ * its encoder (src/model.cpp:402-407).
+ * x, A, B and out of dtype; W of dtype, or e4m3 codes with w_scale (bf16 dtype;
+ * sjh_gemm_fp8w's conditions, and 16-byte aligned A).  bf16 with K a multiple
+ * of 64 and 16-byte aligned tensors and rows of x runs on the bf16 matrix pipes
+ * (x A_a^T rounded to bf16 between the products), all else in fp32 products.
+ * R up to 256, M below 2^24.  act as sjh_gemm's.
+ * workspace: sjh_gemm_lora_workspace(M, R) bytes, 16-byte aligned, free again
+ * once the call's work is done; calls that may overlap (streams, graphs) need
+ * one each.  out overlaps no input. */
+typedef struct sjh_lora_args {
+  const void* x;        /* [M, K] */
+  const void* w;        /* [N, K] */
+  const float* w_scale; /* [N]: w holds e4m3 codes; NULL: w of dtype */
+  const float* bias;    /* [N] or NULL */
+  const void* a;        /* [n_adapters, R, K] */
+  const void* b;        /* [n_adapters, N, R] */
+  const float* scale;   /* [n_adapters], or NULL: 1 */
+  const int32_t* adapter; /* [M], or NULL: adapter 0 for every row */
+  void* out;            /* [M, N] */
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t ld_x, ld_out; /* row strides in elements, 0: K, N */
+  int32_t M, N, K, R, n_adapters, act, dtype;
+} sjh_lora_args;
+int64_t sjh_gemm_lora_workspace(int32_t M, int32_t R);
+int sjh_gemm_lora(const sjh_lora_args* args, sjh_stream_t stream);
+
 /* sj_gemm_geglu (cuda/kernels.cu:168-174): C[M,F] = gelu(A.Wi[:F]^T) * (A.Wi[F:]^T),
  * Wi [2F, K]. */
 int sjh_gemm_geglu(const void* A, const void* Wi, void* C, int32_t M, int32_t F, int32_t K,

@@ -72,6 +72,13 @@ class AddNormArgs(C.Structure):
                 *[(n, C.c_int32) for n in ("post_norm", "pre_norm", "n_gates", "M", "D", "dtype")]]
 
 
+class LoraArgs(C.Structure):
+    """sjh_lora_args: pointers as integers (tensor.data_ptr()) or None."""
+    _fields_ = [*[(n, C.c_void_p) for n in ("x", "w", "w_scale", "bias", "a", "b", "scale", "adapter", "out", "workspace")],
+                *[(n, C.c_int64) for n in ("workspace_bytes", "ld_x", "ld_out")],
+                *[(n, C.c_int32) for n in ("M", "N", "K", "R", "n_adapters", "act", "dtype")]]
+
+
 class AttnScoredArgs(C.Structure):
     """sjh_attn_scored_args: pointers as integers (tensor.data_ptr()) or None."""
     _fields_ = [*[(n, C.c_void_p) for n in ("q", "k", "v", "o", "q_start", "q_len", "k_start", "k_len", "q_pos", "prefix",
@@ -109,6 +116,8 @@ _SIGS = {
     "sjh_quantize_fp8": (C.c_int, [_fp, C.c_int64, C.c_int64, _u8p, _fp]),
     "sjh_gemm_fp8w": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                 C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p]),
+    "sjh_gemm_lora_workspace": (C.c_int64, [C.c_int32, C.c_int32]),
+    "sjh_gemm_lora": (C.c_int, [C.POINTER(LoraArgs), C.c_void_p]),
     "sjh_gemm_geglu": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32,
                                  C.c_int32, C.c_int32, C.c_void_p]),
     "sjh_gemm_residual": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32,

@@ -342,6 +342,67 @@ int sjh_gemm_fp8w(const void* A, const uint8_t* Wq, const float* w_scale, const 
   });
 }
 
+int64_t sjh_gemm_lora_workspace(int32_t M, int32_t R) {
+  if (M < 0 || R < 1 || R > sjh::kLoraMaxRank) {
+    g_last_error = "snapjudge HIP: gemm_lora: M must not be negative and R must lie in [1, 256]";
+    return SJH_E_INVALID;
+  }
+  return sjh::lora_ws_bytes(M, R);
+}
+
+int sjh_gemm_lora(const sjh_lora_args* p, sjh_stream_t stream) {
+  return guarded([&] {
+    using sjh::fail_arg;
+    if (!p) fail_arg("gemm_lora: null arguments");
+    if (p->dtype != SJH_F32 && p->dtype != SJH_BF16) fail_arg("gemm_lora: dtype must be SJH_F32 or SJH_BF16");
+    if (p->act < 0 || p->act > 2) fail_arg("gemm_lora: act must be 0, 1 or 2");
+    if (p->M < 0 || p->N < 0 || p->K < 1) fail_arg("gemm_lora: bad shape");
+    if (p->n_adapters < 0) fail_arg("gemm_lora: negative n_adapters");
+    if (p->n_adapters > 0 && (p->R < 1 || p->R > sjh::kLoraMaxRank)) fail_arg("gemm_lora: R must lie in [1, 256]");
+    if (p->w_scale && p->dtype != SJH_BF16) fail_arg("gemm_lora: fp8 weights need SJH_BF16 rows");
+    const int64_t ldx = p->ld_x ? p->ld_x : p->K, ldo = p->ld_out ? p->ld_out : p->N;
+    if (ldx < p->K || ldo < p->N) fail_arg("gemm_lora: row stride < its row");
+    if (ldo > (1 << 23)) fail_arg("gemm_lora: output row stride above 2^23");  // (32-bit offsets within a tile)
+    if (p->M == 0 || p->N == 0) return;
+    if (!p->x || !p->w || !p->out) fail_arg("gemm_lora: null operand");
+    sjh::LoraArgs l;
+    sjh::GemmArgs& g = l.g;
+    g.A = p->x;
+    g.lda = ldx;
+    g.W = p->w;
+    g.ldw = p->K;
+    g.M = p->M;
+    g.N = p->N;
+    g.K = p->K;
+    g.in_dtype = p->dtype;
+    g.w_dtype = p->w_scale ? sjh::DT_FP8 : p->dtype == SJH_BF16 ? sjh::DT_BF16 : sjh::DT_F32;
+    g.w_scale = p->w_scale;
+    g.out = p->out;
+    g.ldo = ldo;
+    g.out_dtype = p->dtype;
+    g.bias = p->bias;
+    g.act = p->act;
+    if (p->n_adapters == 0) {
+      check_stream(stream);
+      g.epi = sjh::EPI_STORE;
+      sjh::launch_gemm(g, as_stream(stream));
+      return;
+    }
+    if (!p->a || !p->b) fail_arg("gemm_lora: null adapters");
+    if (!p->workspace || p->workspace_bytes < sjh::lora_ws_bytes(p->M, p->R)) fail_arg("gemm_lora: workspace too small");
+    if (reinterpret_cast<uintptr_t>(p->workspace) & 15u) fail_arg("gemm_lora: workspace must be 16-byte aligned");
+    g.lora_b = p->b;
+    g.lora_adapter = p->adapter;
+    g.lora_n = p->n_adapters;
+    g.lora_r = p->R;
+    l.a = p->a;
+    l.scale = p->scale;
+    l.ws = p->workspace;
+    check_stream(stream);
+    sjh::launch_gemm_lora(l, as_stream(stream));
+  });
+}
+
 int sjh_gemm_geglu(const void* A, const void* Wi, void* C, int32_t M, int32_t F, int32_t K,
                    int32_t dtype, sjh_stream_t stream) {
   return guarded([&] {

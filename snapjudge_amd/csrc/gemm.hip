@@ -404,6 +404,72 @@ __device__ __forceinline__ void gemm_epilogue(const GemmArgs& g, f32x16_t (&acc)
   }
 }
 
+// ---- low-rank adapters beside the product (EPI_LORA) -----------------------
+// acc += t . B_a^T for the rows of adapter a: a few more K steps whose operands
+// come straight from memory (t: one 16-byte piece per lane of the row's ranks;
+// B_a: the same of a column's).  Each adapter of a 32-row block (mostly one) has
+// a product of its own, which a row takes where the adapter is its own: zeroed
+// rows of t would do for finite adapters, but one request's infinities must not
+// reach another's rows.  One path for whole and mixed blocks: with a second one
+// that adds onto the accumulators the persistent kernel spills two hundred
+// registers.
+__device__ __forceinline__ bf16x8_t lora_piece(const bf16_t* p, int r, int R, bool vec) {
+  bf16x8_t v = {};
+  if (vec) {
+    if (r < R) v = *reinterpret_cast<const bf16x8_t*>(p + r);
+  } else {
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+      if (r + t < R) v[t] = __builtin_bit_cast(__bf16, p[r + t]);
+  }
+  return v;
+}
+template <int BM, int BN, int WM, int WN, int TI, int TJ, int EPI>
+__device__ __forceinline__ void lora_acc(const GemmArgs& g, f32x16_t (&acc)[TI][TJ], int m0, int tile_n, int wm, int wn,
+                                         int l32, int hb) {
+  const bf16_t* T = static_cast<const bf16_t*>(g.lora_t);
+  const bf16_t* B = static_cast<const bf16_t*>(g.lora_b);
+  const int R = g.lora_r;
+  const bool vec = R % 8 == 0 && (reinterpret_cast<uintptr_t>(B) & 15u) == 0;
+  int64_t wr[TJ];
+#pragma unroll
+  for (int j = 0; j < TJ; ++j) wr[j] = mfma_w_row<BN, WN, EPI>(g, tile_n, wn * WN + j * 32 + l32);
+#pragma unroll
+  for (int i = 0; i < TI; ++i) {
+    const int m = m0 + wm * WM + i * 32 + l32, mc = min(m, g.M - 1);
+    const int ad = g.lora_adapter ? g.lora_adapter[mc] : 0;
+    const bool has = m < g.M && static_cast<unsigned>(ad) < static_cast<unsigned>(g.lora_n);
+    // (both halves of the wave vote alike: the low 32 bits are the rows)
+    uint32_t rest = static_cast<uint32_t>(__ballot(has));
+    const bf16_t* trow = T + static_cast<int64_t>(mc) * g.lora_ld + 8 * hb;
+    while (rest) {
+      const int a = __builtin_amdgcn_readlane(ad, __builtin_ctz(rest));
+      const uint32_t mine = static_cast<uint32_t>(__ballot(has && ad == a));
+      rest &= ~mine;
+      const bf16_t* Ba = B + static_cast<int64_t>(a) * g.N * R;
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) {
+        asm volatile("" ::: "memory");
+        f32x16_t d;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) d[e] = 0.f;
+        for (int r = 0; r < g.lora_ld; r += 16) {
+          const bf16x8_t tf = *reinterpret_cast<const bf16x8_t*>(trow + r);
+          const bf16x8_t bf = lora_piece(Ba + wr[j] * R, r + 8 * hb, R, vec);
+          d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tf, bf, d, 0, 0, 0);
+        }
+        uint32_t sel = mine >> (4 * hb);
+        asm volatile("" : "+v"(sel));
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {  // all ones or zeros from the row's bit: another row's value becomes +0
+          const int on = static_cast<int>(sel << (31 - (8 * (e >> 2) + (e & 3)))) >> 31;
+          acc[i][j][e] += __uint_as_float(__float_as_uint(d[e]) & static_cast<uint32_t>(on));
+        }
+      }
+    }
+  }
+}
+
 // ---- LayerNorm folded across a residual GEMM and the next GEMM -------------
 // (GemmArgs::ln_y / ln_stats_in).  Both sides run in the persistent kernel's
 // direct accumulator layout (lane l holds column l % 32 of each 32x32 block
@@ -1106,6 +1172,8 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_bf16_dma_kernel(GemmArgs 
         for (int e = 0; e < 16; ++e) acc[i][j][e] *= sc;
     }
   }
+  if constexpr (EPI == EPI_LORA)
+    lora_acc<BM, BN, TT::WM, TT::WN, TI, TJ, EPI>(g, acc, m0, tile_n, wm, wn, l32, hb);
   if constexpr (!SPLITK) {
     gemm_epilogue<BM, BN, TT::WM, TT::WN, TI, TJ, EPI, OutT>(g, acc, m0, tile_n, wm, wn, l32, hb);
   } else {
@@ -1765,6 +1833,8 @@ void gemm_bf16_pers_kernel(GemmArgs g0) {
         }
       }
     }
+    if constexpr (EPI == EPI_LORA)
+      lora_acc<BM, BN, TT::WM, TT::WN, TI, TJ, EPI>(g, acc, m0, tn, wme, wne, l32e, hbe);
     if constexpr (LNF == 1)  // A holds folded LayerNorm rows
       ln_fold_acc<BM, BN, TT::WM, TT::WN, TI, TJ, EPI, kSwap>(g, acc, tn, wme, wne, l32e, hbe, fold_tab);
     if constexpr (LNF == 2) {  // the next LayerNorm's input rows and moments too
@@ -1832,6 +1902,9 @@ void launch_pers(const GemmArgs& g, hipStream_t st) {
     case EPI_STORE:
       launch_pers_kernel<BM, BN, WGM, WGN, NS, BK, W8, EPI_STORE, bf16_t, 0>(g, st);
       break;
+    case EPI_LORA:
+      launch_pers_kernel<BM, BN, WGM, WGN, NS, BK, W8, EPI_LORA, bf16_t, 0>(g, st);
+      break;
     case EPI_RESID:
       if constexpr (!W8 && BM == 256 && BN == 256 && WGM == 4 && WGN == 4) {
         if (g.rln_y) {
@@ -1880,6 +1953,7 @@ template <int BM, int BN, int WGM, int WGN, int NS, int BK, bool W8>
 void launch_mfma_epi(const GemmArgs& g, hipStream_t st) {
   switch (g.epi) {
     case EPI_STORE: launch_mfma_tile<BM, BN, WGM, WGN, NS, BK, W8, EPI_STORE>(g, st); break;
+    case EPI_LORA: launch_mfma_tile<BM, BN, WGM, WGN, NS, BK, W8, EPI_LORA>(g, st); break;
     case EPI_RESID: launch_mfma_tile<BM, BN, WGM, WGN, NS, BK, W8, EPI_RESID>(g, st); break;
     case EPI_ROPE: launch_mfma_tile<BM, BN, WGM, WGN, NS, BK, W8, EPI_ROPE>(g, st); break;
     default: launch_mfma_tile<BM, BN, WGM, WGN, NS, BK, W8, EPI_GEGLU>(g, st); break;
@@ -1970,7 +2044,7 @@ Tile pick_tile(const GemmArgs& g) {
   if (count_tiles(g, 128, 64) <= cus) return T128x64;
   const int64_t t128 = count_tiles(g, 128, 128);
   if (t128 <= cus) return T128D;
-  const int short_k = g.w_dtype == DT_FP8 ? 1024 : g.epi == EPI_STORE ? 512 : 256;
+  const int short_k = g.w_dtype == DT_FP8 ? 1024 : g.epi == EPI_STORE || g.epi == EPI_LORA ? 512 : 256;
   if (t128 <= 2 * cus || (g.K <= short_k && 8 * count_tiles(g, 256, 256) < 5 * cus) || !pers_ok(g)) return T128;
   return TPERS;
 }
@@ -1980,6 +2054,7 @@ void launch_mfma(const GemmArgs& g, hipStream_t st) {
   if (!W8 && g.M <= SJH_SMALL32_MAX_M) {
     if (g.epi == EPI_GEGLU) return launch_mfma_tile<SJH_GEMM_SMALL32, false, EPI_GEGLU>(g, st);
     if (g.epi == EPI_STORE) return launch_mfma_tile<SJH_GEMM_SMALL32, false, EPI_STORE>(g, st);
+    if (g.epi == EPI_LORA) return launch_mfma_tile<SJH_GEMM_SMALL32, false, EPI_LORA>(g, st);
     if (g.epi == EPI_ROPE && g.head_dim == 64 && g.N % 64 == 0)
       return launch_mfma_tile<SJH_GEMM_SMALL32, false, EPI_ROPE>(g, st);
   }
@@ -1990,6 +2065,7 @@ void launch_mfma(const GemmArgs& g, hipStream_t st) {
     case T128:  // eight waves where the epilogue also reads (residual rows, RoPE tables)
       switch (g.epi) {
         case EPI_STORE: launch_mfma_tile<128, 128, 2, 2, 2, 64, W8, EPI_STORE>(g, st); break;
+        case EPI_LORA: launch_mfma_tile<128, 128, 2, 2, 2, 64, W8, EPI_LORA>(g, st); break;
         case EPI_GEGLU: launch_mfma_tile<128, 128, 2, 2, 2, 64, W8, EPI_GEGLU>(g, st); break;
         case EPI_RESID: launch_mfma_tile<128, 128, 4, 2, 2, 64, W8, EPI_RESID>(g, st); break;
         default: launch_mfma_tile<128, 128, 4, 2, 2, 64, W8, EPI_ROPE>(g, st); break;
@@ -2144,6 +2220,8 @@ bool mfma_ok(const GemmArgs& g) {
          (g.epi != EPI_ROPE || g.head_dim == 64) && (g.epi != EPI_GEGLU || g.N % 64 == 0);
 }
 
+bool gemm_takes_mfma(const GemmArgs& g) { return g.w_dtype == DT_FP8 || mfma_ok(g); }
+
 bool gemm_takes_ln_fold(const GemmArgs& g) {
   if (g.M <= 0 || g.N <= 0 || g.K <= 0 || !g.A || !g.W) return false;
   if (g.w_dtype == DT_FP8)  // the persistent kernel always (launch_gemm's checks)
@@ -2172,14 +2250,17 @@ int launch_gemm_resid_partials(const GemmArgs& g0, hipStream_t st) {
   return launch_splitk_partials(g, st);
 }
 
-void launch_gemm(const GemmArgs& g, hipStream_t st) {
-  if (g.M <= 0 || g.N <= 0) return;
+void check_gemm(const GemmArgs& g) {
   require(g.K > 0, "gemm: K must be positive");
   require(g.A && g.W, "gemm: null operand");
   require(g.lda >= g.K && g.ldw >= g.K, "gemm: leading dimension < K");
   switch (g.epi) {
     case EPI_STORE:
       require(g.out && g.ldo >= g.N, "gemm: STORE needs out with ldo >= N");
+      break;
+    case EPI_LORA:
+      require(g.out && g.ldo >= g.N && g.lora_t && g.lora_b && g.lora_n > 0 && g.lora_r > 0 && g.lora_ld >= g.lora_r,
+              "gemm: LORA needs out with ldo >= N, adapters and the rows' products with them");
       break;
     case EPI_RESID:
       require(g.X && g.ldx >= g.N, "gemm: RESID needs X with ldx >= N");
@@ -2226,6 +2307,16 @@ void launch_gemm(const GemmArgs& g, hipStream_t st) {
             "gemm: fp8 weights need K % 64 == 0 and 16-byte aligned rows");
     require(pers_ok(g), "gemm: fp8 weights need N % 4 == 0, 16-byte aligned outputs and operands under 4 GiB");
     require(g.epi != EPI_ROPE || g.head_dim == 64, "gemm: fp8 RoPE epilogue needs head_dim 64");
+    return;
+  }
+  require(g.w_dtype == DT_BF16 || g.w_dtype == DT_F32, "gemm: unknown weight type");
+  if (g.epi == EPI_ROPE && !mfma_ok(g)) require(64 % g.head_dim == 0, "gemm: ROPE epilogue needs head_dim dividing 64");
+}
+
+void launch_gemm(const GemmArgs& g, hipStream_t st) {
+  if (g.M <= 0 || g.N <= 0) return;
+  check_gemm(g);
+  if (g.w_dtype == DT_FP8) {
     if (g.epi == EPI_GEGLU && g.N % 64 != 0)
       launch_pers<SJH_GEMM_PERS_FP8, true>(g, st);  // (the other tiles take whole GEGLU columns)
     else
@@ -2233,13 +2324,10 @@ void launch_gemm(const GemmArgs& g, hipStream_t st) {
     check_launch("gemm_fp8w");
     return;
   }
-  require(g.w_dtype == DT_BF16 || g.w_dtype == DT_F32, "gemm: unknown weight type");
   const bool mfma = g.in_dtype == DT_BF16 && (g.out_dtype == DT_BF16 || g.epi == EPI_RESID) &&
                     g.K % kBK == 0 && g.lda % 8 == 0 && g.ldw % 8 == 0 && aligned16(g.A) && aligned16(g.W) &&
                     (g.epi != EPI_ROPE || g.head_dim == 64) &&
                     (g.epi != EPI_GEGLU || g.N % 64 == 0);
-  if (g.epi == EPI_ROPE && !mfma)
-    require(64 % g.head_dim == 0, "gemm: ROPE epilogue needs head_dim dividing 64");
   // split-K only for the residual epilogue: its few output tiles (N = D)
   // leave most CUs idle otherwise; the wider products (QKV, GEGLU) have
   // enough tiles, and a second epilogue kernel costs more than it saves

@@ -44,7 +44,7 @@ namespace sjh {
 namespace {
 
 // ---- epilogue over an fp32 BMxBN tile staged in LDS (row stride ldcs) ----
-template <int BM, int BN, int NT, typename OutT>
+template <int BM, int BN, int NT, typename InT, typename OutT>
 __device__ __forceinline__ void tile_epilogue(const float* Cs, int ldcs, int m0, int tile_n,
                                               const GemmArgs g) {
   const int tid = threadIdx.x;
@@ -91,6 +91,16 @@ __device__ __forceinline__ void tile_epilogue(const float* Cs, int ldcs, int m0,
         if (n < g.rope_dim) v *= g.q_scale;
       }
     } else {
+      if (g.epi == EPI_LORA) {  // the row's fp32 product with its adapter's first matrix
+        const int ad = g.lora_adapter ? g.lora_adapter[m] : 0;
+        if (static_cast<unsigned>(ad) < static_cast<unsigned>(g.lora_n)) {
+          const float* t = static_cast<const float*>(g.lora_t) + static_cast<int64_t>(m) * g.lora_ld;
+          const InT* b = static_cast<const InT*>(g.lora_b) + (static_cast<int64_t>(ad) * g.N + n) * g.lora_r;
+          float d = 0.f;
+          for (int k = 0; k < g.lora_r; ++k) d = __builtin_fmaf(t[k], load_f32(b + k), d);
+          v += d;
+        }
+      }
       if (g.bias) v += g.bias[n];
       if (g.act == 1)
         v = gelu_out<OutT>(v);
@@ -244,7 +254,7 @@ __global__ __launch_bounds__(64 * WGK) void gemm_f32_split_kernel(GemmArgs g0, i
     Cs[o] = v;
   }
   __syncthreads();
-  tile_epilogue<BM, BN, NT, OutT>(Cs, LDC, m0, tile_n, g);
+  tile_epilogue<BM, BN, NT, InT, OutT>(Cs, LDC, m0, tile_n, g);
 }
 
 // BM x 64 tiles, four waves in 2 x 2.  DIRECT (fp32, 16-byte aligned rows): whole
@@ -379,7 +389,7 @@ __global__ __launch_bounds__(256) void gemm_f32_staged_kernel(GemmArgs g0, int v
       for (int e = 0; e < 4; ++e)
         Cs[((wm * TI + i) * 16 + 4 * q + e) * LDC + (wn * TJ + j) * 16 + r16] = acc[i][j][e];
   __syncthreads();
-  tile_epilogue<BM, BN, 256, OutT>(Cs, LDC, m0, tile_n, g);
+  tile_epilogue<BM, BN, 256, InT, OutT>(Cs, LDC, m0, tile_n, g);
 }
 
 unsigned tiles_of(const GemmArgs& g, int BM, int BN) {
@@ -427,7 +437,7 @@ void launch_typed(const GemmArgs& g, hipStream_t st) {
   // 16x16 tiles where 16x64 ones would leave CUs idle and the epilogue (bias,
   // activation, residual) needs no pairs of columns
   const int vec_steps = vec ? g.K / 16 : 0;
-  if (tiles_of(g, 16, 64) < cus && (g.epi == EPI_STORE || g.epi == EPI_RESID))
+  if (tiles_of(g, 16, 64) < cus && (g.epi == EPI_STORE || g.epi == EPI_RESID || g.epi == EPI_LORA))
     gemm_f32_split_kernel<InT, OutT, 1, 8, 6><<<grid_of(tiles_of(g, 16, 16)), 512, 0, st>>>(g, vec_steps);
   else
     gemm_f32_split_kernel<InT, OutT, 4, 8, 6><<<grid_of(tiles_of(g, 16, 64)), 512, 0, st>>>(g, vec_steps);

@@ -18,6 +18,7 @@ enum Epi : int {
   EPI_RESID = 1,  // X (fp32) += acc + bias                (bias optional)
   EPI_ROPE = 2,   // packed (q|k|v) output, rotate-half RoPE on q and k
   EPI_GEGLU = 3,  // out[:, j] = gelu(acc_in[:, j]) * acc_gate[:, j]
+  EPI_LORA = 4,   // out = act(acc + t . lora_b[adapter of the row]^T + bias)  (bias optional)
 };
 
 // out[M, N] = epi(A[M, K] . W[N_w, K]^T).  For EPI_GEGLU, N = F and W is the
@@ -44,6 +45,15 @@ struct GemmArgs {
   int out_dtype = DT_BF16;
   const float* bias = nullptr;  // [N]
   int act = 0;                  // 0 none, 1 erf-GELU, 2 ReLU (STORE)
+  // LORA: t [M, lora_ld] holds each row's scaled product with its adapter's
+  // first matrix (bf16, zero from rank lora_r to lora_ld, for the bf16 and fp8
+  // kernels; fp32 for the fp32-product one; rows without an adapter hold
+  // anything), lora_b [lora_n][N][lora_r] of A's type, lora_adapter [M] (null:
+  // adapter 0; outside [0, lora_n): none)
+  const void* lora_t = nullptr;
+  const void* lora_b = nullptr;
+  const int* lora_adapter = nullptr;
+  int lora_n = 0, lora_r = 0, lora_ld = 0;
   float* X = nullptr;           // RESID
   int64_t ldx = 0;
   const int* pos = nullptr;  // ROPE: position of each row
@@ -112,6 +122,8 @@ constexpr int kLnBlock = 256;
 constexpr bool kLnFoldEnabled = false;
 constexpr int kLnMaxBlocks = 4;  // D <= 1024 (c1 rows hold 8 bf16, blocks past 4 zero)
 void launch_gemm(const GemmArgs& g, hipStream_t st);
+// launch_gemm's checks of its arguments (M, N > 0).
+void check_gemm(const GemmArgs& g);
 // Compute units of the device: launches choose their kernel by how many of its
 // tiles they have per CU.
 int num_cus();
@@ -140,6 +152,20 @@ bool gemm_takes_ln_fold(const GemmArgs& g);
 void launch_ln_fold_consts(const void* W, int w_dtype, const float* w_scale, int n_w, int K,
                            const float* ln_w, const float* ln_b, uint16_t* c1, float* c2,
                            hipStream_t st);
+// sjh_gemm_lora's arguments (include/snapjudge_hip.h), strides filled in: the
+// shared product is g (epi, lora_t and lora_ld are set by the launcher).
+struct LoraArgs {
+  GemmArgs g;
+  const void* a = nullptr;       // [lora_n][lora_r][K] of the rows' type
+  const float* scale = nullptr;  // [lora_n] or null: 1
+  void* ws = nullptr;            // lora_ws_bytes(M, lora_r)
+};
+constexpr int kLoraMaxRank = 256;
+inline int64_t lora_ws_bytes(int M, int R) { return static_cast<int64_t>(M) * ((R + 15) / 16 * 16) * 4; }
+void launch_gemm_lora(const LoraArgs& l, hipStream_t st);
+// Whether launch_gemm takes the bf16 or fp8 kernels for these arguments.
+bool gemm_takes_mfma(const GemmArgs& g);
+
 // Whether the residual epilogue finishes the next LayerNorm for these
 // arguments (GemmArgs::rln_y): the persistent bf16 kernel, N a multiple of 256
 // up to 1024, and at most one tile per workgroup, so that all of a panel's

@@ -127,3 +127,21 @@ def test_attn_scored_workspace_is_a_function_of_the_sizes():
     assert ws(k_rows=9000, max_k=9000, window=50) == 0
     assert ws(k_rows=9000, max_k=9000, B=0) == 0
     assert ws(Dh=7) == -1 and b"head_dim" in sj.lib().sjh_last_error()
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(dtype=2), b"dtype"), (dict(act=3), b"act"), (dict(M=-1), b"bad shape"), (dict(K=0), b"bad shape"), (dict(n_adapters=-1), b"n_adapters"),
+    (dict(R=0), b"R must"), (dict(R=257), b"R must"), (dict(w_scale=16, dtype=sj.SJH_F32), b"fp8"), (dict(ld_x=63), b"stride"), (dict(ld_out=8), b"stride"),
+    (dict(ld_out=(1 << 23) + 1), b"2^23"), (dict(x=None), b"null operand"), (dict(w=None), b"null operand"), (dict(a=None), b"null adapters"),
+    (dict(workspace=None), b"workspace too small"), (dict(workspace_bytes=511), b"workspace too small"), (dict(workspace=24), b"aligned"),
+    (dict(M=1 << 24, workspace_bytes=1 << 40), b"2^24"), (dict(w_scale=16, a=18), b"16-byte aligned adapters"), (dict(w_scale=16, K=72), b"K % 64")])
+def test_gemm_lora_refuses(change, text):
+    kw = dict(x=16, w=16, a=16, b=16, out=16, workspace=16, workspace_bytes=8 * 16 * 4, M=8, N=16, K=64, R=16, n_adapters=2, dtype=sj.SJH_BF16)
+    refused(sj.lib().sjh_gemm_lora, sj.LoraArgs(**{**kw, **change}), text)
+    assert sj.lib().sjh_gemm_lora(None, None) == -1
+
+
+def test_gemm_lora_workspace():
+    ws = sj.lib().sjh_gemm_lora_workspace
+    assert ws(0, 1) == 0 and ws(10, 1) == 10 * 16 * 4 and ws(10, 17) == 10 * 32 * 4
+    assert ws(-1, 4) == -1 and ws(4, 0) == -1 and ws(4, 300) == -1 and b"R must" in sj.lib().sjh_last_error()
