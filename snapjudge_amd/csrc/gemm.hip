@@ -405,14 +405,19 @@ __device__ __forceinline__ void gemm_epilogue(const GemmArgs& g, f32x16_t (&acc)
 }
 
 // ---- low-rank adapters beside the product (EPI_LORA) -----------------------
-// acc += t . B_a^T for the rows of adapter a: a few more K steps whose operands
-// come straight from memory (t: one 16-byte piece per lane of the row's ranks;
-// B_a: the same of a column's).  Each adapter of a 32-row block (mostly one) has
-// a product of its own, which a row takes where the adapter is its own: zeroed
-// rows of t would do for finite adapters, but one request's infinities must not
-// reach another's rows.  One path for whole and mixed blocks: with a second one
-// that adds onto the accumulators the persistent kernel spills two hundred
-// registers.
+// acc += t . B_a^T for the rows of adapter a.
+//
+// EPI_LORAK (bf16 weights): further K stages of the tile kernels' ring
+// (LoraStages below), in which a row of A is the row's t where the stage's
+// columns belong to its adapter and zeros elsewhere, and a row of W is B's.
+// Where a B value that is not finite turns up, those zeros would carry one
+// request's infinities into another's rows: the tile is computed again, operands
+// straight from memory, with lora_acc.
+//
+// EPI_LORA (fp8 weights, and ranks whose rows no 16-byte load reads), lora_acc:
+// after the K loop, operands straight from memory, each adapter of a 32-row
+// block with a product of its own, which a row takes where the adapter is its
+// own.
 __device__ __forceinline__ bf16x8_t lora_piece(const bf16_t* p, int r, int R, bool vec) {
   bf16x8_t v = {};
   if (vec) {
@@ -450,9 +455,7 @@ __device__ __forceinline__ void lora_acc(const GemmArgs& g, f32x16_t (&acc)[TI][
 #pragma unroll
       for (int j = 0; j < TJ; ++j) {
         asm volatile("" ::: "memory");
-        f32x16_t d;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) d[e] = 0.f;
+        f32x16_t d = acc[i][j];
         for (int r = 0; r < g.lora_ld; r += 16) {
           const bf16x8_t tf = *reinterpret_cast<const bf16x8_t*>(trow + r);
           const bf16x8_t bf = lora_piece(Ba + wr[j] * R, r + 8 * hb, R, vec);
@@ -461,14 +464,37 @@ __device__ __forceinline__ void lora_acc(const GemmArgs& g, f32x16_t (&acc)[TI][
         uint32_t sel = mine >> (4 * hb);
         asm volatile("" : "+v"(sel));
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {  // all ones or zeros from the row's bit: another row's value becomes +0
-          const int on = static_cast<int>(sel << (31 - (8 * (e >> 2) + (e & 3)))) >> 31;
-          acc[i][j][e] += __uint_as_float(__float_as_uint(d[e]) & static_cast<uint32_t>(on));
+        for (int e = 0; e < 16; ++e) {  // all ones or zeros from the row's bit
+          const uint32_t on = static_cast<uint32_t>(static_cast<int>(sel << (31 - (8 * (e >> 2) + (e & 3)))) >> 31);
+          acc[i][j][e] = __uint_as_float((__float_as_uint(d[e]) & on) | (__float_as_uint(acc[i][j][e]) & ~on));
         }
       }
     }
   }
 }
+
+// The adapter stages of a tile of BM rows: the tile's distinct adapters, in order
+// of their first rows, side by side along K, C = 2 ceil(R / 16) 16-byte chunks
+// each: whole MFMA steps, so that a row's sum is its K steps', then its own
+// adapter's 16 ranks at a time, and steps that add zeros: the same bits whatever
+// the other rows of the tile are, in any tile shape, and by lora_acc.
+struct LoraStages {
+  int* row_ad;  // LDS [BM]: adapter of each row (any number where it has none)
+  int* list;    // LDS [BM]: the distinct ones
+  int* flag;    // LDS
+  int chunks;   // C
+  // Copies the rows' adapters and the list (made by the launch that made t) into
+  // LDS, 64 of each per wave, before the wave's first stage: landed with it.
+  template <int BM>
+  __device__ __forceinline__ void copy(const GemmArgs& g, int m0, int wave, int lane) const {
+    if (wave < BM / 64) {
+      const int m = min(m0 + 64 * wave + lane, g.M - 1);
+      typedef __attribute__((address_space(3))) void* lds_t;
+      if (g.lora_adapter) __builtin_amdgcn_global_load_lds(g.lora_adapter + m, (lds_t)(row_ad + 64 * wave), 4, 0, 0);
+      __builtin_amdgcn_global_load_lds(lora_list(g) + m, (lds_t)(list + 64 * wave), 4, 0, 0);
+    }
+  }
+};
 
 // ---- LayerNorm folded across a residual GEMM and the next GEMM -------------
 // (GemmArgs::ln_y / ln_stats_in).  Both sides run in the persistent kernel's
@@ -1021,9 +1047,42 @@ struct DTile {
 template <typename OutT>
 __device__ void splitk_output(const GemmArgs& g, int S, int m, int n);
 
+// One WM x WN block of an adapter product by a wave, operands straight from memory in the K order of the staged kernels (the same bits), the adapters
+// by lora_acc: what EPI_LORAK does with a tile that met values that are not finite.
+template <int BM, int BN, int WM, int WN, int TI, int TJ, int EPI, typename OutT>
+__device__ __forceinline__ void lora_redo(const GemmArgs& g, int m0, int tile_n, int wm, int wn, int l32, int hb) {
+  f32x16_t acc[TI][TJ];
+#pragma unroll
+  for (int i = 0; i < TI; ++i)
+#pragma unroll
+    for (int j = 0; j < TJ; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  const bf16_t *a[TI], *w[TJ];
+#pragma unroll
+  for (int i = 0; i < TI; ++i)
+    a[i] = static_cast<const bf16_t*>(g.A) + static_cast<int64_t>(min(m0 + wm * WM + i * 32 + l32, g.M - 1)) * g.lda + 8 * hb;
+#pragma unroll
+  for (int j = 0; j < TJ; ++j)
+    w[j] = static_cast<const bf16_t*>(g.W) + mfma_w_row<BN, WN, EPI>(g, tile_n, wn * WN + j * 32 + l32) * g.ldw + 8 * hb;
+  for (int k = 0; k < g.K; k += 16) {
+    bf16x8_t af[TI], wf[TJ];
+#pragma unroll
+    for (int i = 0; i < TI; ++i) af[i] = *reinterpret_cast<const bf16x8_t*>(a[i] + k);
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) wf[j] = *reinterpret_cast<const bf16x8_t*>(w[j] + k);
+#pragma unroll
+    for (int i = 0; i < TI; ++i)
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[i], wf[j], acc[i][j], 0, 0, 0);
+  }
+  lora_acc<BM, BN, WM, WN, TI, TJ, EPI>(g, acc, m0, tile_n, wm, wn, l32, hb);
+  gemm_epilogue<BM, BN, WM, WN, TI, TJ, EPI, OutT>(g, acc, m0, tile_n, wm, wn, l32, hb);
+}
+
 template <int BM, int BN, int WGM, int WGN, int NS, int BK, int EPI, typename OutT,
           bool SPLITK = false, bool W8 = false>
-__global__ __launch_bounds__(64 * WGM * WGN) void gemm_bf16_dma_kernel(GemmArgs g0) {
+__global__ __launch_bounds__(64 * WGM * WGN, EPI == EPI_LORAK ? (WGM * WGN >= 16 ? 4 : 2) : 1) void gemm_bf16_dma_kernel(GemmArgs g0) {
   using TT = DTile<BM, BN, WGM, WGN, NS, BK, W8>;
   const GemmArgs g = resolve_rows(g0);
   constexpr int TI = TT::TI, TJ = TT::TJ, G = TT::G, RB = TT::RB, CPR = TT::CPR;
@@ -1079,12 +1138,6 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_bf16_dma_kernel(GemmArgs 
   };
 
   f32x16_t acc[TI][TJ];
-#pragma unroll
-  for (int i = 0; i < TI; ++i)
-#pragma unroll
-    for (int j = 0; j < TJ; ++j)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
   // K steps [k_begin, k_begin + nk): all of K, or one split's slice
   int k_begin = 0, nk = g.K / BK;
@@ -1092,21 +1145,82 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_bf16_dma_kernel(GemmArgs 
     k_begin = blockIdx.y * g.k_chunk;
     nk = min(g.k_chunk, nk - k_begin);
   }
+  // adapter stages (bf16 weights) follow the K steps
+  constexpr bool kLoraK = EPI == EPI_LORAK;
+  static_assert(!kLoraK || (BK == 64 && BM % 64 == 0), "an adapter stage is 8 chunks deep");
+  LoraStages ls;
+  int nx = 0;  // of them
+  int n_ad = 0;  // the tile's distinct adapters
+  if constexpr (kLoraK) {
+    int* lds = reinterpret_cast<int*>(dsmem + NS * TT::STAGE_BYTES);
+    ls = LoraStages{lds, lds + BM, lds + 2 * BM, g.lora_ld / 8};
+    n_ad = lora_counts(g)[tile_m];
+    if (tid == 0) *ls.flag = 0;  // (ordered before any wave's vote by the stages' barriers)
+  }
+  // Sources of an adapter stage: 32-bit byte offsets from t and from B.  A row of
+  // another adapter reads the zeros behind t; columns past the list's end, or an
+  // adapter's last ranks, meet zeros of t and read any values of B that there are.
+  // (The swizzle of a lane's rows is the same in all of its groups: one chunk,
+  // one adapter per lane and stage.)
+  static_assert(!kLoraK || TT::NW % 2 == 0, "row groups of a wave differ by a multiple of 16 rows");
+  auto issue_x = [&](int x, int buf) {
+    if constexpr (kLoraK) {
+      char* base = dsmem + buf * TT::STAGE_BYTES;
+      // (lane and wave taken here, where the compiler cannot lift what follows
+      // from them out of the K loop: that cost the 16-wave tile sixty registers)
+      const int lane = lane_id_here(), lrow = lane / CPR, cslot = lane % CPR;
+      int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+      asm volatile("" : "+s"(wave));
+      const int c = 8 * x + (cslot ^ TT::swz(TT::RPI * wave + lrow));
+      const int idx = static_cast<int>((static_cast<float>(c) + 0.5f) * (1.f / static_cast<float>(ls.chunks)));
+      const int ci = c - idx * ls.chunks;
+      const bool real = idx < n_ad;
+      const int ad = ls.list[real ? idx : 0];
+      const uint32_t z = static_cast<uint32_t>(g.M) * static_cast<uint32_t>(g.lora_ld) * 2u;
+      const uint32_t boff = static_cast<uint32_t>(ad) * (static_cast<uint32_t>(g.N) * static_cast<uint32_t>(g.lora_r) * 2u) +
+                            static_cast<uint32_t>(min(8 * ci, g.lora_r - 8)) * 2u;
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        const int q = wave + TT::NW * i, r = TT::RPI * q + lrow;
+        uint32_t off;
+        if (q < BM / TT::RPI) {  // uniform over the wave
+          const bool own = real && (!g.lora_adapter || ls.row_ad[min(r, BM - 1)] == ad);
+          off = own ? static_cast<uint32_t>(min(m0 + r, g.M - 1)) * static_cast<uint32_t>(g.lora_ld) * 2u + static_cast<uint32_t>(ci) * 16u
+                    : z;
+        } else {
+          off = boff + static_cast<uint32_t>(mfma_w_row<BN, TT::WN, EPI>(g, tile_n, r - BM)) * static_cast<uint32_t>(g.lora_r) * 2u;
+        }
+        load_lds16(static_cast<const char*>(q < BM / TT::RPI ? g.lora_t : g.lora_b) + off, base + q * 1024);
+      }
+    }
+  };
+  float nonfin = 0.f;  // NaN once a B value of the wave's is not finite
+#pragma unroll
+  for (int i = 0; i < TI; ++i)
+#pragma unroll
+    for (int j = 0; j < TJ; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  if constexpr (kLoraK) ls.template copy<BM>(g, m0, wave, lane);
 #pragma unroll
   for (int s = 0; s < NS - 1; ++s)
     if (s < nk) issue(k_begin + s, s);
+  if constexpr (kLoraK) {
+    nx = (n_ad * ls.chunks + 7) / 8;
+    if (nk < NS - 1 && nx > 0) {  // few K steps: the first stages are the adapters' too
+      wait_vmcnt<0>();  // (the list)
+      __builtin_amdgcn_s_barrier();
+#pragma unroll
+      for (int s = 0; s < NS - 1; ++s)
+        if (s >= nk && s < nk + nx) issue_x(s - nk, s);
+    }
+  }
 
   // operand rows of this lane; tile bases are multiples of 32, so the
   // swizzle key of row base + l32 is that of l32
   const int xr = TT::swz(l32);
   const int a_row0 = (wm * TT::WM + l32) * RB, w_row0 = BM * RB + (wn * TT::WN + l32) * TT::WRB;
-  for (int kt = 0; kt < nk; ++kt) {
-    if (kt + NS - 2 < nk)
-      wait_vmcnt<G * (NS - 2)>();
-    else
-      wait_vmcnt<0>();
-    __builtin_amdgcn_s_barrier();
-    if (kt + NS - 1 < nk) issue(k_begin + kt + NS - 1, (kt + NS - 1) % NS);
+  auto compute = [&](int kt) {
     const char* sb = dsmem + (kt % NS) * TT::STAGE_BYTES;
     // operand fragments double-buffered across the K steps so the LDS reads
     // of step s + 1 are in flight during the MFMAs of step s
@@ -1160,8 +1274,66 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_bf16_dma_kernel(GemmArgs 
         for (int k = TI * TJ; k < TI + TJ; ++k) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       }
     }
+  };
+  auto stage = [&](int kt, int n) {  // stage kt of n: its loads have landed, the slot of the last one is free
+    if (kt + NS - 2 < n)
+      wait_vmcnt<G * (NS - 2)>();
+    else
+      wait_vmcnt<0>();
+    __builtin_amdgcn_s_barrier();
+  };
+  if constexpr (!kLoraK) {
+    for (int kt = 0; kt < nk; ++kt) {
+      stage(kt, nk);
+      if (kt + NS - 1 < nk) issue(k_begin + kt + NS - 1, (kt + NS - 1) % NS);
+      compute(kt);
+    }
+  } else {
+    // the K steps that only K steps follow, then the rest and the adapters': what
+    // the latter need stays out of the first loop's registers
+    int kt = 0;
+    for (; kt + NS - 1 < nk; ++kt) {
+      stage(kt, nk);
+      issue(kt + NS - 1, (kt + NS - 1) % NS);
+      compute(kt);
+    }
+    const int nt = nk + nx;
+    for (; kt < nt; ++kt) {
+      stage(kt, nt);
+      if (kt + NS - 1 < nt) issue_x(kt + NS - 1 - nk, (kt + NS - 1) % NS);
+      if (kt >= nk) {  // 0 times a B value that is not finite is NaN
+        const char* sb = dsmem + (kt % NS) * TT::STAGE_BYTES;
+                typedef __attribute__((ext_vector_type(2))) __bf16 bf2_t;
+                const bf2_t zero = {};
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+#pragma unroll
+                  for (int j = 0; j < TJ; ++j) {
+                    const bf16x8_t w = *reinterpret_cast<const bf16x8_t*>(sb + w_row0 + j * 32 * RB + ((2 * s + hb) ^ xr) * 16);
+#pragma unroll
+                    for (int t = 0; t < 8; t += 2) nonfin = __builtin_amdgcn_fdot2_f32_bf16((bf2_t){w[t], w[t + 1]}, zero, nonfin, false);
+                  }
+      }
+      compute(kt);
+    }
   }
-
+  if constexpr (kLoraK) {
+    if (nx > 0) {  // uniform: did any wave meet a B value that is not finite
+      if (__any(!(nonfin == 0.f)) && lane == 0) *ls.flag = 1;
+      wait_lgkm0();
+      __builtin_amdgcn_s_barrier();
+      if (*ls.flag) {  // (all indices anew: nothing of this path is computed ahead of the K loop)
+        const int lx = lane_id_here();
+        int wx = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        asm volatile("" : "+s"(wx));
+        // (block by block: its registers must not be what the kernel's budget is spent on)
+#pragma unroll 1
+        for (int b = 0; b < TI * TJ; ++b)
+          lora_redo<BM, BN, 32, 32, 1, 1, EPI, OutT>(g, m0, tile_n, wx / WGN * TI + b / TJ, wx % WGN * TJ + b % TJ, lx & 31, lx >> 5);
+        return;
+      }
+    }
+  }
   if constexpr (W8) {  // row n of W stands for code * w_scale[n]
 #pragma unroll
     for (int j = 0; j < TJ; ++j) {
@@ -1833,8 +2005,6 @@ void gemm_bf16_pers_kernel(GemmArgs g0) {
         }
       }
     }
-    if constexpr (EPI == EPI_LORA)
-      lora_acc<BM, BN, TT::WM, TT::WN, TI, TJ, EPI>(g, acc, m0, tn, wme, wne, l32e, hbe);
     if constexpr (LNF == 1)  // A holds folded LayerNorm rows
       ln_fold_acc<BM, BN, TT::WM, TT::WN, TI, TJ, EPI, kSwap>(g, acc, tn, wme, wne, l32e, hbe, fold_tab);
     if constexpr (LNF == 2) {  // the next LayerNorm's input rows and moments too
@@ -1903,8 +2073,7 @@ void launch_pers(const GemmArgs& g, hipStream_t st) {
       launch_pers_kernel<BM, BN, WGM, WGN, NS, BK, W8, EPI_STORE, bf16_t, 0>(g, st);
       break;
     case EPI_LORA:
-      launch_pers_kernel<BM, BN, WGM, WGN, NS, BK, W8, EPI_LORA, bf16_t, 0>(g, st);
-      break;
+    case EPI_LORAK: fail("gemm: the persistent kernel has no adapter stages");
     case EPI_RESID:
       if constexpr (!W8 && BM == 256 && BN == 256 && WGM == 4 && WGN == 4) {
         if (g.rln_y) {
@@ -1929,7 +2098,8 @@ void launch_pers(const GemmArgs& g, hipStream_t st) {
 
 template <int BM, int BN, int WGM, int WGN, int NS, int BK, bool W8, int EPI, typename OutT>
 void launch_mfma_kernel(const GemmArgs& g, dim3 grid, hipStream_t st) {
-  constexpr int lds = NS * DTile<BM, BN, WGM, WGN, NS, BK, W8>::STAGE_BYTES;
+  constexpr int lds = NS * DTile<BM, BN, WGM, WGN, NS, BK, W8>::STAGE_BYTES +
+                      (EPI == EPI_LORAK ? 8 * BM + 16 : 0);  // (an adapter product's lists)
   auto kern = gemm_bf16_dma_kernel<BM, BN, WGM, WGN, NS, BK, EPI, OutT, false, W8>;
   static bool attr_set = false;  // per instantiation; the attribute is per function
   if (!attr_set) {
@@ -1954,6 +2124,9 @@ void launch_mfma_epi(const GemmArgs& g, hipStream_t st) {
   switch (g.epi) {
     case EPI_STORE: launch_mfma_tile<BM, BN, WGM, WGN, NS, BK, W8, EPI_STORE>(g, st); break;
     case EPI_LORA: launch_mfma_tile<BM, BN, WGM, WGN, NS, BK, W8, EPI_LORA>(g, st); break;
+    case EPI_LORAK:
+      if constexpr (!W8) launch_mfma_tile<BM, BN, WGM, WGN, NS, BK, W8, EPI_LORAK>(g, st);
+      break;
     case EPI_RESID: launch_mfma_tile<BM, BN, WGM, WGN, NS, BK, W8, EPI_RESID>(g, st); break;
     case EPI_ROPE: launch_mfma_tile<BM, BN, WGM, WGN, NS, BK, W8, EPI_ROPE>(g, st); break;
     default: launch_mfma_tile<BM, BN, WGM, WGN, NS, BK, W8, EPI_GEGLU>(g, st); break;
@@ -2044,9 +2217,21 @@ Tile pick_tile(const GemmArgs& g) {
   if (count_tiles(g, 128, 64) <= cus) return T128x64;
   const int64_t t128 = count_tiles(g, 128, 128);
   if (t128 <= cus) return T128D;
-  const int short_k = g.w_dtype == DT_FP8 ? 1024 : g.epi == EPI_STORE || g.epi == EPI_LORA ? 512 : 256;
+  if (g.epi == EPI_LORA) return T128;
+  if (g.epi == EPI_LORAK) return t128 <= 2 * cus ? T128 : TPERS;
+  const int short_k = g.w_dtype == DT_FP8 ? 1024 : g.epi == EPI_STORE ? 512 : 256;
   if (t128 <= 2 * cus || (g.K <= short_k && 8 * count_tiles(g, 256, 256) < 5 * cus) || !pers_ok(g)) return T128;
   return TPERS;
+}
+
+// Rows of the tile that launch_mfma takes for an adapter product.
+int lorak_rows(const GemmArgs& g) {
+  if (g.M <= SJH_SMALL32_MAX_M) return 64;
+  switch (pick_tile(g)) {
+    case T64: return 64;
+    case TPERS: return 256;
+    default: return 128;
+  }
 }
 
 template <bool W8>
@@ -2055,6 +2240,7 @@ void launch_mfma(const GemmArgs& g, hipStream_t st) {
     if (g.epi == EPI_GEGLU) return launch_mfma_tile<SJH_GEMM_SMALL32, false, EPI_GEGLU>(g, st);
     if (g.epi == EPI_STORE) return launch_mfma_tile<SJH_GEMM_SMALL32, false, EPI_STORE>(g, st);
     if (g.epi == EPI_LORA) return launch_mfma_tile<SJH_GEMM_SMALL32, false, EPI_LORA>(g, st);
+    if (g.epi == EPI_LORAK) return launch_mfma_tile<SJH_GEMM_SMALL32, false, EPI_LORAK>(g, st);
     if (g.epi == EPI_ROPE && g.head_dim == 64 && g.N % 64 == 0)
       return launch_mfma_tile<SJH_GEMM_SMALL32, false, EPI_ROPE>(g, st);
   }
@@ -2066,12 +2252,17 @@ void launch_mfma(const GemmArgs& g, hipStream_t st) {
       switch (g.epi) {
         case EPI_STORE: launch_mfma_tile<128, 128, 2, 2, 2, 64, W8, EPI_STORE>(g, st); break;
         case EPI_LORA: launch_mfma_tile<128, 128, 2, 2, 2, 64, W8, EPI_LORA>(g, st); break;
+        case EPI_LORAK:
+          if constexpr (!W8) launch_mfma_tile<128, 128, 2, 2, 2, 64, W8, EPI_LORAK>(g, st);
+          break;
         case EPI_GEGLU: launch_mfma_tile<128, 128, 2, 2, 2, 64, W8, EPI_GEGLU>(g, st); break;
         case EPI_RESID: launch_mfma_tile<128, 128, 4, 2, 2, 64, W8, EPI_RESID>(g, st); break;
         default: launch_mfma_tile<128, 128, 4, 2, 2, 64, W8, EPI_ROPE>(g, st); break;
       }
       break;
     default:
+      if constexpr (!W8)
+        if (g.epi == EPI_LORAK) return launch_mfma_tile<256, 256, 4, 4, 2, 64, W8, EPI_LORAK>(g, st);
       if constexpr (W8)
         launch_pers<SJH_GEMM_PERS_FP8, true>(g, st);
       else
@@ -2220,6 +2411,8 @@ bool mfma_ok(const GemmArgs& g) {
          (g.epi != EPI_ROPE || g.head_dim == 64) && (g.epi != EPI_GEGLU || g.N % 64 == 0);
 }
 
+int gemm_lora_tile_rows(const GemmArgs& g) { return lorak_rows(g); }
+
 bool gemm_takes_mfma(const GemmArgs& g) { return g.w_dtype == DT_FP8 || mfma_ok(g); }
 
 bool gemm_takes_ln_fold(const GemmArgs& g) {
@@ -2259,6 +2452,7 @@ void check_gemm(const GemmArgs& g) {
       require(g.out && g.ldo >= g.N, "gemm: STORE needs out with ldo >= N");
       break;
     case EPI_LORA:
+    case EPI_LORAK:
       require(g.out && g.ldo >= g.N && g.lora_t && g.lora_b && g.lora_n > 0 && g.lora_r > 0 && g.lora_ld >= g.lora_r,
               "gemm: LORA needs out with ldo >= N, adapters and the rows' products with them");
       break;

@@ -19,6 +19,8 @@ enum Epi : int {
   EPI_ROPE = 2,   // packed (q|k|v) output, rotate-half RoPE on q and k
   EPI_GEGLU = 3,  // out[:, j] = gelu(acc_in[:, j]) * acc_gate[:, j]
   EPI_LORA = 4,   // out = act(acc + t . lora_b[adapter of the row]^T + bias)  (bias optional)
+  EPI_LORAK = 5,  // the same, the adapters as further K stages (bf16 operands, lora_r % 8 == 0,
+                  // 16-byte aligned lora_b, t and lora_b under 4 GiB)
 };
 
 // out[M, N] = epi(A[M, K] . W[N_w, K]^T).  For EPI_GEGLU, N = F and W is the
@@ -46,8 +48,8 @@ struct GemmArgs {
   const float* bias = nullptr;  // [N]
   int act = 0;                  // 0 none, 1 erf-GELU, 2 ReLU (STORE)
   // LORA: t [M, lora_ld] holds each row's scaled product with its adapter's
-  // first matrix (bf16, zero from rank lora_r to lora_ld, for the bf16 and fp8
-  // kernels; fp32 for the fp32-product one; rows without an adapter hold
+  // first matrix (bf16, zero from rank lora_r to lora_ld, 16 zero bytes behind
+  // row M - 1, for the bf16 and fp8 kernels; fp32 for the fp32-product one; rows without an adapter hold
   // anything), lora_b [lora_n][N][lora_r] of A's type, lora_adapter [M] (null:
   // adapter 0; outside [0, lora_n): none)
   const void* lora_t = nullptr;
@@ -161,8 +163,16 @@ struct LoraArgs {
   void* ws = nullptr;            // lora_ws_bytes(M, lora_r)
 };
 constexpr int kLoraMaxRank = 256;
-inline int64_t lora_ws_bytes(int M, int R) { return static_cast<int64_t>(M) * ((R + 15) / 16 * 16) * 4; }
+inline int64_t lora_ws_bytes(int M, int R) { return M > 0 ? static_cast<int64_t>(M) * ((R + 15) / 16 * 16) * 4 : 0; }
 void launch_gemm_lora(const LoraArgs& l, hipStream_t st);
+// The workspace of an EPI_LORAK product: t, 16 zero bytes, then (ints) [M] the
+// distinct adapters of each tile of gemm_lora_tile_rows rows, in order of their
+// first rows, from the tile's first row on, and how many of each tile.
+__host__ __device__ inline const int* lora_list(const GemmArgs& g) {
+  return reinterpret_cast<const int*>(static_cast<const char*>(g.lora_t) + static_cast<int64_t>(g.M) * g.lora_ld * 2 + 16);
+}
+__host__ __device__ inline const int* lora_counts(const GemmArgs& g) { return lora_list(g) + g.M; }
+int gemm_lora_tile_rows(const GemmArgs& g);
 // Whether launch_gemm takes the bf16 or fp8 kernels for these arguments.
 bool gemm_takes_mfma(const GemmArgs& g);
 
