@@ -326,31 +326,37 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
             sc[jb][e] = __builtin_fmaf(-slope2, fabsf(d0 - static_cast<float>(key_of(jb, e))), sc[jb][e]);
       }
       if constexpr (PART) {
-        const int pre = s.prefix - base, lo = klo - base, hi = khi - base;
-        if (mk.docs) {
-          const int4* ids = reinterpret_cast<const int4*>(sb + 2 * TILEB) + hb;
+        // (no short cuts: each would be a branch per score; a range of keys is
+        // one unsigned comparison)
+        const int pre = s.prefix - base, lo = klo - base;
+        const uint32_t len = static_cast<uint32_t>(max(khi - klo, 0));
+        auto mask = [&](auto docs_tag, auto pre_tag) {
 #pragma unroll
           for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-              const int4 id = ids[8 * jb + 2 * q];
+              int4 id = {0, 0, 0, 0};
+              if constexpr (decltype(docs_tag)::value) id = reinterpret_cast<const int4*>(sb + 2 * TILEB)[hb + 8 * jb + 2 * q];
               const int dv[4] = {id.x, id.y, id.z, id.w};
 #pragma unroll
               for (int t = 0; t < 4; ++t) {
                 const int k = key_of(jb, 4 * q + t);
-                const bool vis = k < pre || (k >= lo && k < hi && dv[t] == qdoc);
+                bool vis = static_cast<uint32_t>(k - lo) < len;
+                if constexpr (decltype(docs_tag)::value) vis &= dv[t] == qdoc;
+                if constexpr (decltype(pre_tag)::value) vis |= k < pre;
                 sc[jb][4 * q + t] = vis ? sc[jb][4 * q + t] : -INFINITY;
               }
             }
+        };
+        if (mk.docs) {  // uniform
+          if (kt < s.prefix)
+            mask(std::true_type{}, std::true_type{});
+          else
+            mask(std::true_type{}, std::false_type{});
+        } else if (kt < s.prefix) {
+          mask(std::false_type{}, std::true_type{});
         } else {
-#pragma unroll
-          for (int jb = 0; jb < 2; ++jb)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int k = key_of(jb, e);
-              const bool vis = k < pre || (k >= lo && k < hi);
-              sc[jb][e] = vis ? sc[jb][e] : -INFINITY;
-            }
+          mask(std::false_type{}, std::false_type{});
         }
       }
 #pragma unroll
@@ -446,7 +452,7 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[db][e] = 0.f;
     m_i = -INFINITY, l_i = 0.f, l_j = 0.f;
-    TileIter<64 * NW> it(a, s, mk, wg, tile_docs);
+    TileIter<64 * NW> it(a, s, mk, wg, tile_docs, KS ? a.splits * NW : 1, KS ? split * NW + wave_s : 0);
     if constexpr (!KS) {
       int t = it.next(), n = 0;
       int cl = t >= 0 ? it.cls(wr, t) : 0;
@@ -462,19 +468,11 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
       }
     } else {
       // this wave's tiles: every (splits * NW)-th of the list
-      const int stride = a.splits * NW, mine = split * NW + wave_s;
-      int ord = 0;
-      auto next_mine = [&]() {
-        for (;;) {
-          const int t = it.next();
-          if (t < 0 || ord++ % stride == mine) return t;
-        }
-      };
-      int t = next_mine(), n = 0;
+      int t = it.next(), n = 0;
       int cl = t >= 0 ? it.cls(wr, t) : 0;
       if (t >= 0) issue(t, 0);
       while (t >= 0) {
-        const int tn = next_mine();
+        const int tn = it.next();
         const int cn = tn >= 0 ? it.cls(wr, tn) : 0;
         wait_vmcnt<0>();  // (its memory clobber keeps the last tile's reads above the next loads)
         if (tn >= 0) issue(tn, (n + 1) & 1);
@@ -653,6 +651,7 @@ __global__ __launch_bounds__(64 * ks_waves<DH>()) void attn_scored_few_kernel(At
 // Joins the splits of a block: workgroup = block, the rows' sums scaled to the
 // largest offset and added in split order.  T: the output's type; NAT: the
 // offsets are natural logarithms (the fp32-product kernel's), not log2.
+// Grid y: 256 values of the block each.
 template <typename T, bool NAT>
 __global__ __launch_bounds__(256) void attn_scored_merge_kernel(AttnScoredArgs a, int rows) {
   const int G = a.H / a.Hkv, GB = a.pack > 0 ? 1 : G;
@@ -664,25 +663,40 @@ __global__ __launch_bounds__(256) void attn_scored_merge_kernel(AttnScoredArgs a
   const int DH = a.Dh;
   const int64_t pf = part_floats(rows, DH);
   const float* part = a.part + static_cast<int64_t>(item) * a.splits * pf;
-  for (int i = threadIdx.x; i < rows * DH; i += 256) {
-    const int q = i / DH, d = i - q * DH;
-    const int gi = a.pack > 0 ? q / a.max_q : 0;
-    const int oq = a.pack > 0 ? q - gi * a.max_q : qb * rows + q;
-    if (gi >= G || oq >= s.qlen) continue;
-    const float* pm = part + static_cast<int64_t>(rows) * DH + q;
-    float M = -INFINITY;
-    for (int k = 0; k < a.splits; ++k) M = fmaxf(M, pm[k * pf]);
-    float l = 0.f, x = 0.f;
-    for (int k = 0; k < a.splits; ++k) {
-      const float mk = pm[k * pf];
-      const float f = mk == -INFINITY ? 1.f : NAT ? expf(mk - M) : __builtin_amdgcn_exp2f(mk - M);
-      l += pm[k * pf + rows] * f;
-      x += part[k * pf + i] * f;
+  const int i = blockIdx.y * 256 + threadIdx.x;
+  if (i >= rows * DH) return;
+  const int q = i / DH, d = i - q * DH;
+  const int gi = a.pack > 0 ? q / a.max_q : 0;
+  const int oq = a.pack > 0 ? q - gi * a.max_q : qb * rows + q;
+  if (gi >= G || oq >= s.qlen) return;
+  // eight splits' loads at a time, the sums rescaled to the larger offset between
+  const float* pm = part + static_cast<int64_t>(rows) * DH + q;
+  auto ex = [](float y) { return NAT ? expf(y) : __builtin_amdgcn_exp2f(y); };
+  float M = -INFINITY, l = 0.f, x = 0.f;
+  constexpr int U = 8;
+  for (int k0 = 0; k0 < a.splits; k0 += U) {
+    float mk[U], lk[U], xk[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t o = min(k0 + u, a.splits - 1) * pf;
+      mk[u] = pm[o], lk[u] = pm[o + rows], xk[u] = part[o + i];
     }
-    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-    const int oh = kvh * G + (a.pack > 0 ? gi : g);
-    store_f32(static_cast<T*>(a.o) + (s.q_row + oq) * a.ld_o + static_cast<int64_t>(oh) * DH + d, x * inv);
+    float Mn = M;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (k0 + u < a.splits) Mn = fmaxf(Mn, mk[u]);
+    const float f0 = M == -INFINITY ? 1.f : ex(M - Mn);
+    l *= f0, x *= f0, M = Mn;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (k0 + u < a.splits) {
+        const float f = mk[u] == -INFINITY ? 1.f : ex(mk[u] - M);
+        l += lk[u] * f, x += xk[u] * f;
+      }
   }
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+  const int oh = kvh * G + (a.pack > 0 ? gi : g);
+  store_f32(static_cast<T*>(a.o) + (s.q_row + oq) * a.ld_o + static_cast<int64_t>(oh) * DH + d, x * inv);
 }
 
 // How a launch is cut: from its sizes alone, for a device of 256 CUs.
@@ -780,7 +794,7 @@ void launch_attn_scored(const AttnScoredArgs& a0, hipStream_t st) {
     launch_dh<128>(a, p, st);
   check_launch("attn_scored");
   if (p.splits > 1) {
-    const unsigned n = static_cast<unsigned>(p.items);
+    const dim3 n(static_cast<unsigned>(p.items), static_cast<unsigned>((p.rows * a.Dh + 255) / 256));
     if (p.mfma)
       attn_scored_merge_kernel<bf16_t, false><<<n, 256, 0, st>>>(a, p.rows);
     else if (a.dtype == DT_BF16)

@@ -104,16 +104,15 @@ __global__ __launch_bounds__(256) void attn_scored_f32_kernel(AttnScoredArgs a, 
 #pragma unroll
     for (int t = 0; t < ND; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     m_i = -INFINITY, l_i = 0.f;
-    TileIter<256> it(a, s, mk, wg, tile_docs);
-    int ord = 0, tl = -1, cls = 0, half = HALVES - 1;
+    TileIter<256> it(a, s, mk, wg, tile_docs, a.splits, split);
+    int tl = -1, cls = 0, half = HALVES - 1;
     // next step: (key offset, or -1; masks needed)
     auto next = [&](int& kt, int& cl) {
       if (++half < HALVES && tl >= 0 && tl * kTile + half * KT < s.klen) {
         kt = tl * kTile + half * KT, cl = cls;
         return;
       }
-      do tl = it.next();
-      while (tl >= 0 && ord++ % a.splits != split);
+      tl = it.next();
       half = 0;
       if (tl >= 0) cls = it.cls(wg, tl);
       kt = tl >= 0 ? tl * kTile : -1, cl = cls;

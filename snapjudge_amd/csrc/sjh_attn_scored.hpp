@@ -96,11 +96,14 @@ struct TileIter {
   const Masks& m;
   const QRange& wg;  // the workgroup's queries
   int2* tile_docs;   // LDS, 64 entries
+  int stride, mine;
   uint64_t mask = 0;
   int word = -1, t0 = 0, t1 = 0;  // lane t: documents of tile 64 word + t
+  int before = 0;                 // entries of earlier words
 
-  __device__ __forceinline__ TileIter(const AttnScoredArgs& a_, const Seq& s_, const Masks& m_, const QRange& wg_, int2* td)
-      : a(a_), s(s_), m(m_), wg(wg_), tile_docs(td) {}
+  __device__ __forceinline__ TileIter(const AttnScoredArgs& a_, const Seq& s_, const Masks& m_, const QRange& wg_, int2* td,
+                                      int stride_ = 1, int mine_ = 0)
+      : a(a_), s(s_), m(m_), wg(wg_), tile_docs(td), stride(stride_), mine(mine_) {}
 
   __device__ __forceinline__ void eval() {
     const int lane = threadIdx.x & 63;
@@ -132,9 +135,17 @@ struct TileIter {
       const int2 d = tile_docs[lane];
       t0 = d.x, t1 = d.y;
     }
-    mask = __ballot(k0 < m.klen && m.need(wg, k0, t0, t1));
+    const bool need = k0 < m.klen && m.need(wg, k0, t0, t1);
+    mask = __ballot(need);
+    if (stride > 1) {
+      const int rank = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32),
+                                                 __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
+      const int total = before + __builtin_popcountll(mask);
+      mask = __ballot(need && (before + rank) % stride == mine);
+      before = total;
+    }
   }
-  // Tile of the next entry, or -1.
+  // Tile of the next entry of its own, or -1.
   __device__ __forceinline__ int next() {
     while (mask == 0) {
       if ((word + 1) * 64 * kTile >= m.klen) return -1;
