@@ -81,6 +81,9 @@ __device__ __forceinline__ void lds_read_tr4(s16x4_t (&r)[4], uint32_t a0, uint3
       : "memory");
 }
 
+enum Cap : int { CAP_NONE = 0, CAP_FIXED = 1, CAP_ANY = 2 };
+constexpr float kFixedCap = 96.f;
+
 // Redo passes: how a V value enters the product.
 enum VMode : int {
   V_FINITE = 0,    // infinities and NaN as 0
@@ -111,8 +114,14 @@ __device__ __forceinline__ bf16x8_t v_map(bf16x8_t v, int mode) {
 
 // The work of workgroup (pair of sequence and key head, head of the group,
 // query block, split).  NW waves; KS: the waves (and splits) divide the keys.
-template <int DH, int NW, bool KS, bool CAP, bool BIAS>
+template <int DH, int NW, bool KS, int CAPM, bool BIAS>
 __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem, int b, int kvh, int g, int qb, int split) {
+  constexpr bool CAP = CAPM != CAP_NONE;
+  // Capped scores without a bias lie within [-cap, cap]: with the cap at most
+  // kFixedCap in log2, weights 2^s need no running maximum (8192 of them and
+  // their products stay far inside fp32 and bf16).
+  constexpr bool FIXED = CAPM == CAP_FIXED;
+  static_assert(!FIXED || !BIAS, "a bias leaves no lower bound");
   constexpr int ROWB = DH * 2, TILEB = kTile * ROWB;          // bytes of a row, of a K or V tile
   constexpr int STAGE = 2 * TILEB + 256;                      // K, V, the keys' documents
   constexpr int RPI = 1024 / ROWB;                            // rows per load instruction
@@ -230,7 +239,7 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
         vaddr[db][hl] = lds_addr(ring) + TILEB + t_off<DH>(8 * hl + 4 * (tg >> 1) + tk, db * 32 + 16 * (tg & 1) + 4 * tq);
   }
 
-  const float slope2 = BIAS ? a.slopes[head] * kLog2e : 0.f;
+  const float slope2 = BIAS && a.slopes ? a.slopes[head] * kLog2e : 0.f;
   const float c = a.scale * kLog2e;                     // plain scores to log2
   const float cap2 = CAP ? a.softcap * kLog2e : 0.f;    // the cap in log2
   const float ucap = CAP ? a.scale / a.softcap : 0.f;   // u = ucap raw
@@ -248,38 +257,59 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
     return __builtin_fmaf(w, __builtin_fmaf(w, __builtin_fmaf(w, A3, A2), A1), A0);
   };
 
-  f32x16_t o[DB];
-  float m_i, l_i, l_j;
-
-  // One tile from ring slot `slot`.  PART: masks; NF: V through v_map(mode).
-  auto tile = [&](auto part_tag, auto nf_tag, int mode, int slot, int tl) {
-    constexpr bool PART = decltype(part_tag)::value, NF = decltype(nf_tag)::value;
-    const char* sb = ring + slot * STAGE;
-    const int kt = tl * kTile;
-    f32x16_t sc[2];
-#pragma unroll
-    for (int jb = 0; jb < 2; ++jb) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) sc[jb][e] = 0.f;
-    }
-    if constexpr (DH == 64) {
-      bf16x8_t kf[2][ST];
+  // Bias of a tile that lies on one side of all of the wave's queries: slope (key
+  // - pos), or its negative, is linear in the key, so a 16-deep MFMA step adds the
+  // part within the tile to the scores: the key's offset (whole numbers up to 63,
+  // exact in bf16) times slope / scale as three bf16 summands, and the tile's
+  // part joins the softmax offset.  The matrix pipe has the time; on the vector
+  // pipe it is two instructions per score.
+  constexpr bool LIN = BIAS && !CAP;
+  bf16x8_t sf = {}, ko[2] = {};
+  if constexpr (LIN) {
+    const float r = (a.slopes ? a.slopes[head] : 0.f) / a.scale;
+    const __bf16 h0 = static_cast<__bf16>(r), h1 = static_cast<__bf16>(r - static_cast<float>(h0));
+    const __bf16 h2 = static_cast<__bf16>(r - static_cast<float>(h0) - static_cast<float>(h1));
+    if (hb == 0) {
+      sf[0] = h0, sf[1] = h1, sf[2] = h2;
 #pragma unroll
       for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
-        for (int st = 0; st < ST; ++st) kf[jb][st] = *reinterpret_cast<const bf16x8_t*>(sb + jb * (32 * ROWB) + koff[st]);
+        for (int t = 0; t < 3; ++t) ko[jb][t] = static_cast<__bf16>(static_cast<float>(32 * jb + l32));
+    }
+  }
+
+  f32x16_t o[DB];
+  float m_i, l_i, l_j;
+
+  // One tile from ring slot `slot`.  PART: masks; NF: V through v_map(mode).  side
+  // (whole tiles under a linear bias): 1 keys before the queries, 3 after.
+  auto tile = [&](auto part_tag, auto nf_tag, int mode, int slot, int tl, int side) {
+    constexpr bool PART = decltype(part_tag)::value, NF = decltype(nf_tag)::value;
+    const char* sb = ring + slot * STAGE;
+    const int kt = tl * kTile;
+    constexpr bool LINT = LIN && !PART;
+    f32x16_t sc[2];
+    const f32x16_t zero16 = {};
+    if constexpr (LINT) {
+      u32x4_t s4 = __builtin_bit_cast(u32x4_t, sf);
+      const uint32_t flip = side == 3 ? 0x80008000u : 0u;
+      s4[0] ^= flip, s4[1] ^= flip;
 #pragma unroll
-      for (int st = 0; st < ST; ++st)
+      for (int jb = 0; jb < 2; ++jb)
+        sc[jb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ko[jb], __builtin_bit_cast(bf16x8_t, s4), zero16, 0, 0, 0);
+    }
+    bf16x8_t kf[2][4];
 #pragma unroll
-        for (int jb = 0; jb < 2; ++jb) sc[jb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[jb][st], qf[st], sc[jb], 0, 0, 0);
-    } else {
+    for (int s0 = 0; s0 < ST; s0 += 4) {
 #pragma unroll
-      for (int st = 0; st < ST; ++st)
+      for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
-        for (int jb = 0; jb < 2; ++jb) {
-          const bf16x8_t kf = *reinterpret_cast<const bf16x8_t*>(sb + jb * (32 * ROWB) + koff[st]);
-          sc[jb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[st], sc[jb], 0, 0, 0);
-        }
+        for (int st = 0; st < 4; ++st) kf[jb][st] = *reinterpret_cast<const bf16x8_t*>(sb + jb * (32 * ROWB) + koff[s0 + st]);
+#pragma unroll
+      for (int st = 0; st < 4; ++st)
+#pragma unroll
+        for (int jb = 0; jb < 2; ++jb)
+          sc[jb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[jb][st], qf[s0 + st], !LINT && s0 + st == 0 ? zero16 : sc[jb], 0, 0, 0);
     }
     // element (jb, e) is key kt + 4 hb + key_of(jb, e)
     auto key_of = [](int jb, int e) { return 32 * jb + 8 * (e >> 2) + (e & 3); };
@@ -294,15 +324,17 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
       small = !__any(!(amax <= raw_max));
     }
     // FUSED: the cap's last product and the softmax offset meet in one FMA
-    constexpr bool FUSED = !PART && !BIAS;
+    constexpr bool FUSED = !PART && (!BIAS || LINT);
+    const float tb = LINT ? slope2 * static_cast<float>(side == 3 ? pos - kt : kt - pos) : 0.f;  // the tile's bias
     float tmax = -INFINITY;
-    if constexpr (FUSED) {
+    if constexpr (FUSED && FIXED) {
+    } else if constexpr (FUSED) {
 #pragma unroll
       for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
         for (int e = 0; e < 16; ++e) tmax = fmaxf(tmax, sc[jb][e]);
       tmax = wave_max32(tmax);
-      tmax = CAP ? cap_exact(tmax) : tmax * c;  // both rise with the score
+      tmax = CAP ? cap_exact(tmax) : __builtin_fmaf(tmax, c, tb);  // both rise with the score
     } else {
       const float d0 = static_cast<float>(pos - base);
       if (!CAP || small) {
@@ -328,9 +360,12 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
       if constexpr (PART) {
         // (no short cuts: each would be a branch per score; a range of keys is
         // one unsigned comparison)
-        const int pre = s.prefix - base, lo = klo - base;
         const uint32_t len = static_cast<uint32_t>(max(khi - klo, 0));
         auto mask = [&](auto docs_tag, auto pre_tag) {
+          int pre = s.prefix - base, lo = klo - base;
+          // (each form's own: the compiler would compute the comparisons that the
+          // forms share ahead of the branch and hold 32 of them)
+          asm volatile("" : "+v"(lo), "+v"(pre));
 #pragma unroll
           for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
@@ -359,48 +394,54 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
           mask(std::false_type{}, std::false_type{});
         }
       }
+      if constexpr (!FIXED) {
 #pragma unroll
-      for (int jb = 0; jb < 2; ++jb)
+        for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) tmax = fmaxf(tmax, sc[jb][e]);
-      tmax = wave_max32(tmax);
+          for (int e = 0; e < 16; ++e) tmax = fmaxf(tmax, sc[jb][e]);
+        tmax = wave_max32(tmax);
+      }
     }
     // the running max, raised only when the tile's exceeds it by more than
     // kLazy (weights stay below 2^kLazy; the quotient is exact either way)
-    const bool bump = tmax > m_i + kLazy;
-    if (__any(bump)) {
-      asm volatile("" ::: "memory");  // a branch (rarely taken), not a select
-      const float m_new = bump ? tmax : m_i;
-      const float alpha = m_i == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_i - m_new);
-      m_i = m_new;
-      l_i *= alpha;
-      l_j *= alpha;
+    if constexpr (!FIXED) {
+      const bool bump = tmax > m_i + kLazy;
+      if (__any(bump)) {
+        asm volatile("" ::: "memory");  // a branch (rarely taken), not a select
+        const float m_new = bump ? tmax : m_i;
+        const float alpha = m_i == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_i - m_new);
+        m_i = m_new;
+        l_i *= alpha;
+        l_j *= alpha;
 #pragma unroll
-      for (int db = 0; db < DB; ++db)
+        for (int db = 0; db < DB; ++db)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[db][e] *= alpha;
+          for (int e = 0; e < 16; ++e) o[db][e] *= alpha;
+      }
     }
-    const float m_use = m_i == -INFINITY ? 0.f : m_i;
+    const float m_use = FIXED || m_i == -INFINITY ? 0.f : m_i;
     if constexpr (FUSED) {
+      const float off = LINT ? tb - m_use : -m_use;  // (0 under a fixed offset: a product instead of the FMA)
       if (!CAP || small) {
         if constexpr (CAP) asm volatile("" ::: "memory");
 #pragma unroll
         for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            sc[jb][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[jb][e], CAP ? cap_poly(sc[jb][e]) : c, -m_use));
+            sc[jb][e] = __builtin_amdgcn_exp2f(FIXED ? sc[jb][e] * cap_poly(sc[jb][e])
+                                                     : __builtin_fmaf(sc[jb][e], CAP ? cap_poly(sc[jb][e]) : c, off));
       } else {
         asm volatile("" ::: "memory");
 #pragma unroll
         for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) sc[jb][e] = __builtin_amdgcn_exp2f(cap_exact(sc[jb][e]) - m_use);
+          for (int e = 0; e < 16; ++e) sc[jb][e] = __builtin_amdgcn_exp2f(FIXED ? cap_exact(sc[jb][e]) : cap_exact(sc[jb][e]) - m_use);
       }
     } else {
 #pragma unroll
       for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sc[jb][e] = __builtin_amdgcn_exp2f(sc[jb][e] - m_use);
+        for (int e = 0; e < 16; ++e) sc[jb][e] = __builtin_amdgcn_exp2f(FIXED ? sc[jb][e] : sc[jb][e] - m_use);
     }
     // O^T += V^T P^T.  The MFMA's k index 8 hb + t of 16-key step g stands for
     // key 16 g + 4 hb + t (t < 4) or 16 g + 8 + 4 hb + t - 4, as the S^T
@@ -440,26 +481,33 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
   int* flag = reinterpret_cast<int*>(tile_docs + 64);
   auto run = [&](int cl, auto nf_tag, int mode, int slot, int t) {
     if constexpr (!decltype(nf_tag)::value)
-      if (cl == 1) {
-        tile(std::false_type{}, nf_tag, mode, slot, t);
+      if (cl & 1) {
+        tile(std::false_type{}, nf_tag, mode, slot, t, cl);
         return;
       }
-    tile(std::true_type{}, nf_tag, mode, slot, t);  // (a redo masks every tile: one body of its own)
+    tile(std::true_type{}, nf_tag, mode, slot, t, cl);  // (a redo masks every tile: one body of its own)
+  };
+  // a tile's class for the wave: 0 nothing, 2 masks, 1 whole (3 whole, behind the
+  // queries; under a linear bias only a tile on one side counts as whole)
+  auto class_of = [&](const auto& it, int t) {
+    const int cl = it.cls(wr, t);
+    if (!LIN || cl != 1) return cl;
+    return t * kTile + kTile - 1 <= wr.p0 ? 1 : t * kTile >= wr.p1 ? 3 : 2;
   };
   auto pass = [&](auto nf_tag, int mode) {
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[db][e] = 0.f;
-    m_i = -INFINITY, l_i = 0.f, l_j = 0.f;
+    m_i = FIXED ? 0.f : -INFINITY, l_i = 0.f, l_j = 0.f;
     TileIter<64 * NW> it(a, s, mk, wg, tile_docs, KS ? a.splits * NW : 1, KS ? split * NW + wave_s : 0);
     if constexpr (!KS) {
       int t = it.next(), n = 0;
-      int cl = t >= 0 ? it.cls(wr, t) : 0;
+      int cl = t >= 0 ? class_of(it, t) : 0;
       if (t >= 0) issue(t, 0);
       while (t >= 0) {
         const int tn = it.next();  // (its barriers, if any, before the loads are waited for)
-        const int cn = tn >= 0 ? it.cls(wr, tn) : 0;
+        const int cn = tn >= 0 ? class_of(it, tn) : 0;
         wait_vmcnt<0>();
         __builtin_amdgcn_s_barrier();
         if (tn >= 0) issue(tn, (n + 1) & 1);
@@ -469,11 +517,11 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
     } else {
       // this wave's tiles: every (splits * NW)-th of the list
       int t = it.next(), n = 0;
-      int cl = t >= 0 ? it.cls(wr, t) : 0;
+      int cl = t >= 0 ? class_of(it, t) : 0;
       if (t >= 0) issue(t, 0);
       while (t >= 0) {
         const int tn = it.next();
-        const int cn = tn >= 0 ? it.cls(wr, tn) : 0;
+        const int cn = tn >= 0 ? class_of(it, tn) : 0;
         wait_vmcnt<0>();  // (its memory clobber keeps the last tile's reads above the next loads)
         if (tn >= 0) issue(tn, (n + 1) & 1);
         run(cl, nf_tag, mode, n & 1, t);
@@ -610,8 +658,8 @@ constexpr int lds_bytes() {
 // Query blocks of 128.  Workgroup i runs on XCD i % 8: the blocks and heads
 // that read one key head go to one XCD, close together, where the pairs fill
 // the XCDs evenly enough (a.pack is then 0; -1: blocks in plain order).
-template <int DH, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, DH == 64 ? 2 : 1) void attn_scored_kernel(AttnScoredArgs a) {
+template <int DH, int CAP, bool BIAS>
+__global__ __launch_bounds__(256, DH == 64 ? 3 : 2) void attn_scored_kernel(AttnScoredArgs a) {
   __shared__ __attribute__((aligned(16))) char smem[lds_bytes<DH, 4, false>()];
   const int G = a.H / a.Hkv, per = G * a.n_blocks;
   int pair, r;
@@ -637,7 +685,7 @@ template <int DH>
 constexpr int ks_waves() {
   return DH == 64 ? 4 : 2;
 }
-template <int DH, bool CAP, bool BIAS>
+template <int DH, int CAP, bool BIAS>
 __global__ __launch_bounds__(64 * ks_waves<DH>()) void attn_scored_few_kernel(AttnScoredArgs a) {
   constexpr int NW = ks_waves<DH>();
   __shared__ __attribute__((aligned(16))) char smem[lds_bytes<DH, NW, true>()];
@@ -746,7 +794,7 @@ Plan plan_of(const AttnScoredArgs& a) {
   return p;
 }
 
-template <int DH, bool CAP, bool BIAS>
+template <int DH, int CAP, bool BIAS>
 void launch_mfma(const AttnScoredArgs& a, const Plan& p, hipStream_t st) {
   if (p.few) {
     attn_scored_few_kernel<DH, CAP, BIAS>
@@ -766,10 +814,12 @@ void launch_mfma(const AttnScoredArgs& a, const Plan& p, hipStream_t st) {
 
 template <int DH>
 void launch_dh(const AttnScoredArgs& a, const Plan& p, hipStream_t st) {
-  if (a.softcap > 0.f)
-    a.slopes ? launch_mfma<DH, true, true>(a, p, st) : launch_mfma<DH, true, false>(a, p, st);
+  if (!(a.softcap > 0.f))
+    a.slopes ? launch_mfma<DH, CAP_NONE, true>(a, p, st) : launch_mfma<DH, CAP_NONE, false>(a, p, st);
+  else if (!a.slopes && a.softcap * kLog2e <= kFixedCap)
+    launch_mfma<DH, CAP_FIXED, false>(a, p, st);
   else
-    a.slopes ? launch_mfma<DH, false, true>(a, p, st) : launch_mfma<DH, false, false>(a, p, st);
+    launch_mfma<DH, CAP_ANY, true>(a, p, st);  // (no slopes: a bias of 0)
 }
 
 }  // namespace
