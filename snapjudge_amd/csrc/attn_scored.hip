@@ -46,7 +46,12 @@ namespace sjh {
 namespace {
 
 constexpr float kLazy = 8.f;  // log2 headroom before the running max is raised
-constexpr int kNS = 2;        // ring stages
+// Ring stages: a workgroup's shared ring, two stages ahead of the one in use where
+// three workgroups of them fit a CU (head_dim 64); one ahead else.
+template <int DH, bool KS>
+constexpr int ring_stages() {
+  return DH == 64 && !KS ? 3 : 2;
+}
 
 // tanh(u) = u (c0 + c1 u^2 + c2 u^4 + c3 u^6) + e, |e| < 6e-7 for |u| <= 0.6
 // (a least-squares fit over the interval, reweighted to even out the error):
@@ -131,7 +136,8 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
   constexpr int NL = GRP / LW;                                // ... per wave, K and V each
   constexpr int ST = DH / 16, DB = DH / 32;                   // K steps of QK^T, 32-dim blocks
   constexpr int QB = KS ? 32 : 32 * NW;                       // queries of the workgroup
-  constexpr int RING = kNS * STAGE;                           // bytes of a ring
+  constexpr int NS = ring_stages<DH, KS>();
+  constexpr int RING = NS * STAGE;                            // bytes of a ring
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int wave_s = __builtin_amdgcn_readfirstlane(wave);
   const int l32 = lane & 31, hb = lane >> 5;
@@ -217,7 +223,7 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
       load_lds16_buf(rk, koffs[i], 0u, base + grp * 1024);
       load_lds16_buf(rv, voffs[i], 0u, base + TILEB + grp * 1024);
     }
-    if (kdoc && (KS || wave_s == 0))
+    if (kdoc)  // (every wave the same 64: the count of loads per stage is one for all)
       __builtin_amdgcn_global_load_lds(kdoc + min(k0 + lane, s.klen - 1),
                                        (__attribute__((address_space(3))) void*)(base + 2 * TILEB), 4, 0, 0);
   };
@@ -361,7 +367,7 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
         // (no short cuts: each would be a branch per score; a range of keys is
         // one unsigned comparison)
         const uint32_t len = static_cast<uint32_t>(max(khi - klo, 0));
-        auto mask = [&](auto docs_tag, auto pre_tag) {
+        auto mask = [&](auto docs_tag, auto pre_tag, auto range_tag) {
           int pre = s.prefix - base, lo = klo - base;
           // (each form's own: the compiler would compute the comparisons that the
           // forms share ahead of the branch and hold 32 of them)
@@ -376,22 +382,29 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
 #pragma unroll
               for (int t = 0; t < 4; ++t) {
                 const int k = key_of(jb, 4 * q + t);
-                bool vis = static_cast<uint32_t>(k - lo) < len;
+                bool vis = true;
+                if constexpr (decltype(range_tag)::value) vis = static_cast<uint32_t>(k - lo) < len;
                 if constexpr (decltype(docs_tag)::value) vis &= dv[t] == qdoc;
                 if constexpr (decltype(pre_tag)::value) vis |= k < pre;
                 sc[jb][4 * q + t] = vis ? sc[jb][4 * q + t] : -INFINITY;
               }
             }
         };
-        if (mk.docs) {  // uniform
+        // (uniform) the documents alone decide where nothing else reaches the tile
+        const bool range = a.window || a.causal || kt + kTile > s.klen;
+        using Y = std::true_type;
+        using N = std::false_type;
+        if (mk.docs) {
           if (kt < s.prefix)
-            mask(std::true_type{}, std::true_type{});
+            mask(Y{}, Y{}, Y{});
+          else if (range)
+            mask(Y{}, N{}, Y{});
           else
-            mask(std::true_type{}, std::false_type{});
+            mask(Y{}, N{}, N{});
         } else if (kt < s.prefix) {
-          mask(std::false_type{}, std::true_type{});
+          mask(N{}, Y{}, Y{});
         } else {
-          mask(std::false_type{}, std::false_type{});
+          mask(N{}, N{}, Y{});
         }
       }
       if constexpr (!FIXED) {
@@ -502,17 +515,30 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
     m_i = FIXED ? 0.f : -INFINITY, l_i = 0.f, l_j = 0.f;
     TileIter<64 * NW> it(a, s, mk, wg, tile_docs, KS ? a.splits * NW : 1, KS ? split * NW + wave_s : 0);
     if constexpr (!KS) {
-      int t = it.next(), n = 0;
-      int cl = t >= 0 ? class_of(it, t) : 0;
-      if (t >= 0) issue(t, 0);
-      while (t >= 0) {
-        const int tn = it.next();  // (its barriers, if any, before the loads are waited for)
-        const int cn = tn >= 0 ? class_of(it, tn) : 0;
-        wait_vmcnt<0>();
+      // the tile in use and the NS - 1 after it, with their classes
+      int tq[NS], cq[NS], slot = 0;
+#pragma unroll
+      for (int i = 0; i < NS - 1; ++i) {
+        tq[i] = it.next();
+        cq[i] = tq[i] >= 0 ? class_of(it, tq[i]) : 0;
+        if (tq[i] >= 0) issue(tq[i], i);
+      }
+      while (tq[0] >= 0) {
+        tq[NS - 1] = it.next();  // (its barriers, if any, before the loads are waited for)
+        cq[NS - 1] = tq[NS - 1] >= 0 ? class_of(it, tq[NS - 1]) : 0;
+        if (NS == 2 || tq[1] < 0)
+          wait_vmcnt<0>();
+        else if (kdoc)
+          wait_vmcnt<(NS - 2) * (2 * NL + 1)>();
+        else
+          wait_vmcnt<(NS - 2) * 2 * NL>();
         __builtin_amdgcn_s_barrier();
-        if (tn >= 0) issue(tn, (n + 1) & 1);
-        if (wave_active && cl != 0) run(cl, nf_tag, mode, n & 1, t);
-        t = tn, cl = cn, ++n;
+        const int last = slot == 0 ? NS - 1 : slot - 1;  // the slot that the tile before was in
+        if (tq[NS - 1] >= 0) issue(tq[NS - 1], last);
+        if (wave_active && cq[0] != 0) run(cq[0], nf_tag, mode, slot, tq[0]);
+        slot = slot == NS - 1 ? 0 : slot + 1;
+#pragma unroll
+        for (int i = 0; i < NS - 1; ++i) tq[i] = tq[i + 1], cq[i] = cq[i + 1];
       }
     } else {
       // this wave's tiles: every (splits * NW)-th of the list
@@ -652,7 +678,7 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
 // LDS: the ring or rings, the list's documents, the redo flag.
 template <int DH, int NW, bool KS>
 constexpr int lds_bytes() {
-  return (KS ? NW : 1) * kNS * (2 * kTile * DH * 2 + 256) + 64 * 8 + 16;
+  return (KS ? NW : 1) * ring_stages<DH, KS>() * (2 * kTile * DH * 2 + 256) + 64 * 8 + 16;
 }
 
 // Query blocks of 128.  Workgroup i runs on XCD i % 8: the blocks and heads
@@ -666,6 +692,10 @@ __global__ __launch_bounds__(256, DH == 64 ? 3 : 2) void attn_scored_kernel(Attn
   if (a.pack < 0) {
     pair = blockIdx.x / per;
     r = blockIdx.x - pair * per;
+  } else if (a.causal) {  // the longest rows of all of the XCD's pairs first
+    const int xcd = blockIdx.x & 7, kx = blockIdx.x >> 3, np = (a.B * a.Hkv + 7) / 8;
+    r = kx / np;
+    pair = xcd + 8 * (kx - r * np);
   } else {
     const int xcd = blockIdx.x & 7, kx = blockIdx.x >> 3;
     pair = xcd + 8 * (kx / per);
@@ -675,7 +705,7 @@ __global__ __launch_bounds__(256, DH == 64 ? 3 : 2) void attn_scored_kernel(Attn
   const int b = pair / a.Hkv, kvh = pair - b * a.Hkv;
   int qb = r / G;
   const int g = r - qb * G;
-  if (a.causal) qb = a.n_blocks - 1 - qb;  // the long rows first
+  if (a.causal) qb = a.n_blocks - 1 - qb;
   scored_item<DH, 4, false, CAP, BIAS>(a, smem, b, kvh, g, qb, 0);
 }
 
