@@ -182,12 +182,17 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
   }
   if (mk.docs) doc_range(a, s, q0, n_wg, wg.d0, wg.d1);
   if constexpr (KS) wr = wg;
-  const int qdoc = mk.docs ? a.q_doc[qrow] : 0;
-  // keys [klo, khi) are those of the lane's window and past
-  const int klo = a.window ? pos - a.window : 0;
-  int khi = s.klen;
-  if (a.window) khi = min(khi, pos + a.window + 1);
-  if (a.causal) khi = min(khi, pos + 1);
+  // what masks and biases ask of the lane's query, in LDS: needed by some tiles
+  // only, and spilled registers would be reloaded behind the ring's loads
+  int4* qinfo = reinterpret_cast<int4*>(smem + (KS ? NW : 1) * RING + 64 * 8 + 16) + wave * 32 + l32;
+  {
+    // {position, first key and number of keys of the lane's window and past, document}
+    const int klo = a.window ? pos - a.window : 0;
+    int khi = s.klen;
+    if (a.window) khi = min(khi, pos + a.window + 1);
+    if (a.causal) khi = min(khi, pos + 1);
+    *qinfo = make_int4(pos, klo, max(khi - klo, 0), mk.docs ? a.q_doc[qrow] : 0);
+  }
 
   const bf16_t* Q = static_cast<const bf16_t*>(a.q) + static_cast<int64_t>(head) * DH;
   const bf16_t* K = static_cast<const bf16_t*>(a.k) + s.k_row * a.ld_k + static_cast<int64_t>(kvh) * DH;
@@ -245,15 +250,19 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
         vaddr[db][hl] = lds_addr(ring) + TILEB + t_off<DH>(8 * hl + 4 * (tg >> 1) + tk, db * 32 + 16 * (tg & 1) + 4 * tq);
   }
 
-  const float slope2 = BIAS && a.slopes ? a.slopes[head] * kLog2e : 0.f;
-  const float c = a.scale * kLog2e;                     // plain scores to log2
-  const float cap2 = CAP ? a.softcap * kLog2e : 0.f;    // the cap in log2
-  const float ucap = CAP ? a.scale / a.softcap : 0.f;   // u = ucap raw
+  // constants of the launch (and, but for packed heads, the head's slope) in
+  // scalar registers: the vector ones are what the tile's code is short of
+  auto uni = [](float x) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x))); };
+  const float slope1 = BIAS && a.slopes ? a.slopes[head] * kLog2e : 0.f;
+  const float slope2 = KS ? slope1 : uni(slope1);
+  const float c = uni(a.scale * kLog2e);                     // plain scores to log2
+  const float cap2 = uni(CAP ? a.softcap * kLog2e : 0.f);    // the cap in log2
+  const float ucap = CAP ? a.scale / a.softcap : 0.f;        // u = ucap raw
   // y = raw (A0 + w (A1 + w (A2 + w A3))), w = raw^2
-  const float A0 = cap2 * ucap * kTanh0, A1 = cap2 * ucap * ucap * ucap * kTanh1;
-  const float A2 = A1 / kTanh1 * ucap * ucap * kTanh2, A3 = A2 / kTanh2 * ucap * ucap * kTanh3;
-  const float raw_max = CAP && fabsf(A3) < INFINITY ? kTanhMax / ucap : -1.f;
-  const float kexp = 2.f * kLog2e * ucap;
+  const float B0 = cap2 * ucap, B1 = B0 * ucap * ucap, B2 = B1 * ucap * ucap, B3 = B2 * ucap * ucap;
+  const float A0 = uni(B0 * kTanh0), A1 = uni(B1 * kTanh1), A2 = uni(B2 * kTanh2), A3 = uni(B3 * kTanh3);
+  const float raw_max = uni(CAP && fabsf(A3) < INFINITY ? kTanhMax / ucap : -1.f);
+  const float kexp = uni(2.f * kLog2e * ucap);
   auto cap_exact = [&](float x) {  // cap2 tanh(ucap x), any x
     const float e = __builtin_amdgcn_exp2f(x * kexp);
     return __builtin_fmaf(-2.f * cap2, __builtin_amdgcn_rcpf(1.f + e), cap2);
@@ -270,39 +279,37 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
   // part joins the softmax offset.  The matrix pipe has the time; on the vector
   // pipe it is two instructions per score.
   constexpr bool LIN = BIAS && !CAP;
-  bf16x8_t sf = {}, ko[2] = {};
+  uint32_t sf0 = 0, sf1 = 0;  // the summands, packed; the operands are made from them per tile
   if constexpr (LIN) {
     const float r = (a.slopes ? a.slopes[head] : 0.f) / a.scale;
-    const __bf16 h0 = static_cast<__bf16>(r), h1 = static_cast<__bf16>(r - static_cast<float>(h0));
-    const __bf16 h2 = static_cast<__bf16>(r - static_cast<float>(h0) - static_cast<float>(h1));
-    if (hb == 0) {
-      sf[0] = h0, sf[1] = h1, sf[2] = h2;
-#pragma unroll
-      for (int jb = 0; jb < 2; ++jb)
-#pragma unroll
-        for (int t = 0; t < 3; ++t) ko[jb][t] = static_cast<__bf16>(static_cast<float>(32 * jb + l32));
-    }
+    const float r1 = r - bf16_to_f32(f32_to_bf16(r)), r2 = r1 - bf16_to_f32(f32_to_bf16(r1));
+    if (hb == 0) sf0 = pack_bf16x2(r, r1), sf1 = pack_bf16x2(r2, 0.f);
   }
 
   f32x16_t o[DB];
   float m_i, l_i, l_j;
 
-  // One tile from ring slot `slot`.  PART: masks; NF: V through v_map(mode).  side
-  // (whole tiles under a linear bias): 1 keys before the queries, 3 after.
-  auto tile = [&](auto part_tag, auto nf_tag, int mode, int slot, int tl, int side) {
-    constexpr bool PART = decltype(part_tag)::value, NF = decltype(nf_tag)::value;
+  // One tile from ring slot `slot`.  PART: masks.  MAXR: the running maximum; else
+  // weights are 2^s as they come (pass_check).  NF: V through v_map(mode) where
+  // mode >= 0.  side (whole tiles under a linear bias): 1 keys before the queries,
+  // 3 after.
+  auto tile = [&](auto part_tag, auto max_tag, auto nf_tag, int mode, int slot, int tl, int side) {
+    constexpr bool PART = decltype(part_tag)::value, NF = decltype(nf_tag)::value, NOMAX = !decltype(max_tag)::value;
     const char* sb = ring + slot * STAGE;
     const int kt = tl * kTile;
     constexpr bool LINT = LIN && !PART;
     f32x16_t sc[2];
     const f32x16_t zero16 = {};
     if constexpr (LINT) {
-      u32x4_t s4 = __builtin_bit_cast(u32x4_t, sf);
       const uint32_t flip = side == 3 ? 0x80008000u : 0u;
-      s4[0] ^= flip, s4[1] ^= flip;
+      const u32x4_t s4 = {sf0 ^ flip, sf1 ^ flip, 0u, 0u};
 #pragma unroll
-      for (int jb = 0; jb < 2; ++jb)
-        sc[jb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ko[jb], __builtin_bit_cast(bf16x8_t, s4), zero16, 0, 0, 0);
+      for (int jb = 0; jb < 2; ++jb) {
+        // (the upper half of the wave meets zeros of s4: only its summands 0 to 2 count)
+        const uint32_t o1 = __float_as_uint(static_cast<float>(32 * jb + l32)) >> 16;
+        const u32x4_t k4 = {o1 | o1 << 16, o1, 0u, 0u};
+        sc[jb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, k4), __builtin_bit_cast(bf16x8_t, s4), zero16, 0, 0, 0);
+      }
     }
     bf16x8_t kf[2][4];
 #pragma unroll
@@ -331,9 +338,13 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
     }
     // FUSED: the cap's last product and the softmax offset meet in one FMA
     constexpr bool FUSED = !PART && (!BIAS || LINT);
-    const float tb = LINT ? slope2 * static_cast<float>(side == 3 ? pos - kt : kt - pos) : 0.f;  // the tile's bias
+    float tb = 0.f;  // the tile's bias
+    if constexpr (LINT) {
+      const int qp = qinfo->x;
+      tb = slope2 * static_cast<float>(side == 3 ? qp - kt : kt - qp);
+    }
     float tmax = -INFINITY;
-    if constexpr (FUSED && FIXED) {
+    if constexpr (FUSED && NOMAX) {
     } else if constexpr (FUSED) {
 #pragma unroll
       for (int jb = 0; jb < 2; ++jb)
@@ -342,7 +353,8 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
       tmax = wave_max32(tmax);
       tmax = CAP ? cap_exact(tmax) : __builtin_fmaf(tmax, c, tb);  // both rise with the score
     } else {
-      const float d0 = static_cast<float>(pos - base);
+      const int4 qi4 = *qinfo;
+      const float d0 = static_cast<float>(qi4.x - base);
       if (!CAP || small) {
         if constexpr (CAP) asm volatile("" ::: "memory");  // a branch, not a select
 #pragma unroll
@@ -366,9 +378,10 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
       if constexpr (PART) {
         // (no short cuts: each would be a branch per score; a range of keys is
         // one unsigned comparison)
-        const uint32_t len = static_cast<uint32_t>(max(khi - klo, 0));
+        const uint32_t len = static_cast<uint32_t>(qi4.z);
+        const int qdoc = qi4.w;
         auto mask = [&](auto docs_tag, auto pre_tag, auto range_tag) {
-          int pre = s.prefix - base, lo = klo - base;
+          int pre = s.prefix - base, lo = qi4.y - base;
           // (each form's own: the compiler would compute the comparisons that the
           // forms share ahead of the branch and hold 32 of them)
           asm volatile("" : "+v"(lo), "+v"(pre));
@@ -407,7 +420,7 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
           mask(N{}, N{}, Y{});
         }
       }
-      if constexpr (!FIXED) {
+      if constexpr (!NOMAX) {
 #pragma unroll
         for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
@@ -417,7 +430,7 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
     }
     // the running max, raised only when the tile's exceeds it by more than
     // kLazy (weights stay below 2^kLazy; the quotient is exact either way)
-    if constexpr (!FIXED) {
+    if constexpr (!NOMAX) {
       const bool bump = tmax > m_i + kLazy;
       if (__any(bump)) {
         asm volatile("" ::: "memory");  // a branch (rarely taken), not a select
@@ -432,7 +445,7 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
           for (int e = 0; e < 16; ++e) o[db][e] *= alpha;
       }
     }
-    const float m_use = FIXED || m_i == -INFINITY ? 0.f : m_i;
+    const float m_use = NOMAX || m_i == -INFINITY ? 0.f : m_i;
     if constexpr (FUSED) {
       const float off = LINT ? tb - m_use : -m_use;  // (0 under a fixed offset: a product instead of the FMA)
       if (!CAP || small) {
@@ -441,20 +454,21 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
         for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            sc[jb][e] = __builtin_amdgcn_exp2f(FIXED ? sc[jb][e] * cap_poly(sc[jb][e])
+            sc[jb][e] = __builtin_amdgcn_exp2f(NOMAX && CAP ? sc[jb][e] * cap_poly(sc[jb][e])
+                                               : NOMAX && !LINT ? sc[jb][e] * c
                                                      : __builtin_fmaf(sc[jb][e], CAP ? cap_poly(sc[jb][e]) : c, off));
       } else {
         asm volatile("" ::: "memory");
 #pragma unroll
         for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) sc[jb][e] = __builtin_amdgcn_exp2f(FIXED ? cap_exact(sc[jb][e]) : cap_exact(sc[jb][e]) - m_use);
+          for (int e = 0; e < 16; ++e) sc[jb][e] = __builtin_amdgcn_exp2f(NOMAX ? cap_exact(sc[jb][e]) : cap_exact(sc[jb][e]) - m_use);
       }
     } else {
 #pragma unroll
       for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sc[jb][e] = __builtin_amdgcn_exp2f(FIXED ? sc[jb][e] : sc[jb][e] - m_use);
+        for (int e = 0; e < 16; ++e) sc[jb][e] = __builtin_amdgcn_exp2f(NOMAX ? sc[jb][e] : sc[jb][e] - m_use);
     }
     // O^T += V^T P^T.  The MFMA's k index 8 hb + t of 16-key step g stands for
     // key 16 g + 4 hb + t (t < 4) or 16 g + 8 + 4 hb + t - 4, as the S^T
@@ -482,7 +496,8 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
         for (int d = 0; d < 2; ++d) {
           const s16x4_t lo = vr[2 * d], hi = vr[2 * d + 1];
           bf16x8_t vf = __builtin_bit_cast(bf16x8_t, (s16x8_t){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
-          if constexpr (NF) vf = v_map(vf, mode);
+          if constexpr (NF)
+            if (mode >= 0) vf = v_map(vf, mode);
           o[2 * dp + d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf, o[2 * dp + d], 0, 0, 0);
         }
       }
@@ -492,13 +507,19 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
   // One pass over the needed tiles.
   int2* tile_docs = reinterpret_cast<int2*>(smem + (KS ? NW : 1) * RING);
   int* flag = reinterpret_cast<int*>(tile_docs + 64);
-  auto run = [&](int cl, auto nf_tag, int mode, int slot, int t) {
-    if constexpr (!decltype(nf_tag)::value)
-      if (cl & 1) {
-        tile(std::false_type{}, nf_tag, mode, slot, t, cl);
-        return;
-      }
-    tile(std::true_type{}, nf_tag, mode, slot, t, cl);  // (a redo masks every tile: one body of its own)
+  // REDO: a pass again, with the running maximum and (mode >= 0) V mapped; it masks
+  // every tile, so that it has one body of its own.  Few queries (KS) keep the
+  // maximum at first too: what a wave or split holds is not the whole row.
+  auto run = [&](int cl, auto redo_tag, int mode, int slot, int t) {
+    using Y = std::true_type;
+    using N = std::false_type;
+    using Max = std::integral_constant<bool, KS>;
+    if constexpr (decltype(redo_tag)::value)
+      tile(Y{}, Y{}, Y{}, mode, slot, t, cl);
+    else if (cl & 1)
+      tile(N{}, Max{}, N{}, mode, slot, t, cl);
+    else
+      tile(Y{}, Max{}, N{}, mode, slot, t, cl);
   };
   // a tile's class for the wave: 0 nothing, 2 masks, 1 whole (3 whole, behind the
   // queries; under a linear bias only a tile on one side counts as whole)
@@ -507,12 +528,13 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
     if (!LIN || cl != 1) return cl;
     return t * kTile + kTile - 1 <= wr.p0 ? 1 : t * kTile >= wr.p1 ? 3 : 2;
   };
-  auto pass = [&](auto nf_tag, int mode) {
+  auto pass = [&](auto redo_tag, int mode) {
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[db][e] = 0.f;
-    m_i = FIXED ? 0.f : -INFINITY, l_i = 0.f, l_j = 0.f;
+    constexpr bool kMax = KS || decltype(redo_tag)::value;
+    m_i = kMax ? -INFINITY : 0.f, l_i = 0.f, l_j = 0.f;
     TileIter<64 * NW> it(a, s, mk, wg, tile_docs, KS ? a.splits * NW : 1, KS ? split * NW + wave_s : 0);
     if constexpr (!KS) {
       // the tile in use and the NS - 1 after it, with their classes
@@ -535,7 +557,7 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
         __builtin_amdgcn_s_barrier();
         const int last = slot == 0 ? NS - 1 : slot - 1;  // the slot that the tile before was in
         if (tq[NS - 1] >= 0) issue(tq[NS - 1], last);
-        if (wave_active && cq[0] != 0) run(cq[0], nf_tag, mode, slot, tq[0]);
+        if (wave_active && cq[0] != 0) run(cq[0], redo_tag, mode, slot, tq[0]);
         slot = slot == NS - 1 ? 0 : slot + 1;
 #pragma unroll
         for (int i = 0; i < NS - 1; ++i) tq[i] = tq[i + 1], cq[i] = cq[i + 1];
@@ -550,7 +572,7 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
         const int cn = tn >= 0 ? class_of(it, tn) : 0;
         wait_vmcnt<0>();  // (its memory clobber keeps the last tile's reads above the next loads)
         if (tn >= 0) issue(tn, (n + 1) & 1);
-        run(cl, nf_tag, mode, n & 1, t);
+        run(cl, redo_tag, mode, n & 1, t);
         t = tn, cl = cn, ++n;
       }
     }
@@ -559,18 +581,40 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
     __syncthreads();  // every wave is done with the ring and the list
   };
   if (tid == 0) *flag = 0;  // ordered before other waves' writes by the pass's last barrier
-  pass(std::false_type{}, V_FINITE);
-  {
-    // an output that is not finite: a visible key's value, or a masked one's
-    // times a weight of 0
+  pass(std::false_type{}, -1);
+  auto vote = [&](bool bad) {  // whether any wave's
+    if (__any(bad && live) && lane == 0) *flag = 1;
+    __syncthreads();
+    const bool any = *flag != 0;
+    __syncthreads();
+    if (any && tid == 0) *flag = 0;
+    return any;
+  };
+  // an output that is not finite: a visible key's value, or a masked one's times
+  // a weight of 0
+  auto unclean = [&] {
     bool bad = false;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
       for (int e = 0; e < 16; ++e) bad |= !(fabsf(o[db][e]) < INFINITY);
-    if (__any(bad && live) && lane == 0) *flag = 1;
-    __syncthreads();
-    if (*flag) {  // uniform over the workgroup
+    return bad;
+  };
+  {
+    // Without the maximum (pass_check): every row's weight sum must lie in [2^-60,
+    // 2^64].  Then nothing overflowed, and a weight that flushed to zero (below
+    // 2^-126) is under 2^-50 of the largest.  Else (a row that sees no key
+    // among them, but for scores that a cap bounds) the workgroup runs again with
+    // the maximum, as it does for an output that is not finite.
+    bool again = unclean();
+    if constexpr (!KS && !FIXED) again |= !(l_i >= 0x1p-60f && l_i <= 0x1p64f);
+    if (vote(again)) {  // uniform over the workgroup
+      pass(std::true_type{}, -1);
+      again = vote(unclean());
+    } else {
+      again = false;
+    }
+    if (again) {
       // which outputs saw a value that is not finite, and whether any but
       // +inf, any but -inf; then the sums of the finite ones
       uint32_t saw[3][DB / 2] = {};
@@ -675,10 +719,10 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
   }
 }
 
-// LDS: the ring or rings, the list's documents, the redo flag.
+// LDS: the ring or rings, the list's documents, the redo flag, the queries' masks.
 template <int DH, int NW, bool KS>
 constexpr int lds_bytes() {
-  return (KS ? NW : 1) * ring_stages<DH, KS>() * (2 * kTile * DH * 2 + 256) + 64 * 8 + 16;
+  return (KS ? NW : 1) * ring_stages<DH, KS>() * (2 * kTile * DH * 2 + 256) + 64 * 8 + 16 + 32 * NW * 16;
 }
 
 // Query blocks of 128.  Workgroup i runs on XCD i % 8: the blocks and heads
