@@ -360,13 +360,17 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
 #pragma unroll
         for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) sc[jb][e] *= CAP ? cap_poly(sc[jb][e]) : c;
+          for (int e = 0; e < 16; ++e) {
+            sc[jb][e] *= CAP ? cap_poly(sc[jb][e]) : c;
+          }
       } else {
         asm volatile("" ::: "memory");
 #pragma unroll
         for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) sc[jb][e] = cap_exact(sc[jb][e]);
+          for (int e = 0; e < 16; ++e) {
+            sc[jb][e] = cap_exact(sc[jb][e]);
+          }
       }
       if constexpr (BIAS) {
 #pragma unroll
@@ -453,16 +457,19 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
 #pragma unroll
         for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
+          for (int e = 0; e < 16; ++e) {
             sc[jb][e] = __builtin_amdgcn_exp2f(NOMAX && CAP ? sc[jb][e] * cap_poly(sc[jb][e])
                                                : NOMAX && !LINT ? sc[jb][e] * c
                                                      : __builtin_fmaf(sc[jb][e], CAP ? cap_poly(sc[jb][e]) : c, off));
+          }
       } else {
         asm volatile("" ::: "memory");
 #pragma unroll
         for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) sc[jb][e] = __builtin_amdgcn_exp2f(NOMAX ? cap_exact(sc[jb][e]) : cap_exact(sc[jb][e]) - m_use);
+          for (int e = 0; e < 16; ++e) {
+            sc[jb][e] = __builtin_amdgcn_exp2f(NOMAX ? cap_exact(sc[jb][e]) : cap_exact(sc[jb][e]) - m_use);
+          }
       }
     } else {
 #pragma unroll
@@ -510,13 +517,14 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
   // REDO: a pass again, with the running maximum and (mode >= 0) V mapped; it masks
   // every tile, so that it has one body of its own.  Few queries (KS) keep the
   // maximum at first too: what a wave or split holds is not the whole row.
-  auto run = [&](int cl, auto redo_tag, int mode, int slot, int t) {
+  // WHOLE: the tile needs no masks.
+  auto run = [&](int cl, auto whole_tag, auto redo_tag, int mode, int slot, int t) {
     using Y = std::true_type;
     using N = std::false_type;
     using Max = std::integral_constant<bool, KS>;
     if constexpr (decltype(redo_tag)::value)
       tile(Y{}, Y{}, Y{}, mode, slot, t, cl);
-    else if (cl & 1)
+    else if constexpr (decltype(whole_tag)::value)
       tile(N{}, Max{}, N{}, mode, slot, t, cl);
     else
       tile(Y{}, Max{}, N{}, mode, slot, t, cl);
@@ -524,6 +532,7 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
   // a tile's class for the wave: 0 nothing, 2 masks, 1 whole (3 whole, behind the
   // queries; under a linear bias only a tile on one side counts as whole)
   auto class_of = [&](const auto& it, int t) {
+    if (!wave_active) return 0;
     const int cl = it.cls(wr, t);
     if (!LIN || cl != 1) return cl;
     return t * kTile + kTile - 1 <= wr.p0 ? 1 : t * kTile >= wr.p1 ? 3 : 2;
@@ -545,7 +554,7 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
         cq[i] = tq[i] >= 0 ? class_of(it, tq[i]) : 0;
         if (tq[i] >= 0) issue(tq[i], i);
       }
-      while (tq[0] >= 0) {
+      auto step = [&](auto whole_tag) {
         tq[NS - 1] = it.next();  // (its barriers, if any, before the loads are waited for)
         cq[NS - 1] = tq[NS - 1] >= 0 ? class_of(it, tq[NS - 1]) : 0;
         if (NS == 2 || tq[1] < 0)
@@ -557,23 +566,35 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
         __builtin_amdgcn_s_barrier();
         const int last = slot == 0 ? NS - 1 : slot - 1;  // the slot that the tile before was in
         if (tq[NS - 1] >= 0) issue(tq[NS - 1], last);
-        if (wave_active && cq[0] != 0) run(cq[0], redo_tag, mode, slot, tq[0]);
+        if (cq[0] != 0) run(cq[0], whole_tag, redo_tag, mode, slot, tq[0]);
         slot = slot == NS - 1 ? 0 : slot + 1;
 #pragma unroll
         for (int i = 0; i < NS - 1; ++i) tq[i] = tq[i + 1], cq[i] = cq[i + 1];
+      };
+      // runs of whole tiles and of others, a loop each: one loop with a branch
+      // between the two bodies copies the accumulators on every tile
+      while (tq[0] >= 0) {
+        if constexpr (!decltype(redo_tag)::value)
+          while (tq[0] >= 0 && (cq[0] & 1)) step(std::true_type{});
+        while (tq[0] >= 0 && (decltype(redo_tag)::value || !(cq[0] & 1))) step(std::false_type{});
       }
     } else {
       // this wave's tiles: every (splits * NW)-th of the list
       int t = it.next(), n = 0;
       int cl = t >= 0 ? class_of(it, t) : 0;
       if (t >= 0) issue(t, 0);
-      while (t >= 0) {
+      auto step = [&](auto whole_tag) {
         const int tn = it.next();
         const int cn = tn >= 0 ? class_of(it, tn) : 0;
         wait_vmcnt<0>();  // (its memory clobber keeps the last tile's reads above the next loads)
         if (tn >= 0) issue(tn, (n + 1) & 1);
-        run(cl, redo_tag, mode, n & 1, t);
+        run(cl, whole_tag, redo_tag, mode, n & 1, t);
         t = tn, cl = cn, ++n;
+      };
+      while (t >= 0) {
+        if constexpr (!decltype(redo_tag)::value)
+          while (t >= 0 && (cl & 1)) step(std::true_type{});
+        while (t >= 0 && (decltype(redo_tag)::value || !(cl & 1))) step(std::false_type{});
       }
     }
     l_i += l_j;
