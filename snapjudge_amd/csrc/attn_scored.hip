@@ -47,10 +47,13 @@ namespace {
 
 constexpr float kLazy = 8.f;  // log2 headroom before the running max is raised
 // Ring stages: a workgroup's shared ring, two stages ahead of the one in use where
-// three workgroups of them fit a CU (head_dim 64); one ahead else.
+// three workgroups of them fit a CU (head_dim 64), one ahead else; a wave's own,
+// one ahead at head_dim 64, none at 128 (four waves' stages fill the LDS, and
+// the waves cover one another: 3 x 8191 keys, 4 key heads, 19.2 us with two waves
+// and a stage ahead).
 template <int DH, bool KS>
 constexpr int ring_stages() {
-  return DH == 64 && !KS ? 3 : 2;
+  return KS ? (DH == 64 ? 2 : 1) : (DH == 64 ? 3 : 2);
 }
 
 // tanh(u) = u (c0 + c1 u^2 + c2 u^4 + c3 u^6) + e, |e| < 6e-7 for |u| <= 0.6
@@ -587,8 +590,13 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
         const int tn = it.next();
         const int cn = tn >= 0 ? class_of(it, tn) : 0;
         wait_vmcnt<0>();  // (its memory clobber keeps the last tile's reads above the next loads)
-        if (tn >= 0) issue(tn, (n + 1) & 1);
-        run(cl, whole_tag, redo_tag, mode, n & 1, t);
+        if (NS > 1 && tn >= 0) issue(tn, (n + 1) % NS);
+        run(cl, whole_tag, redo_tag, mode, n % NS, t);
+        if (NS == 1 && tn >= 0) {
+          wait_lgkm0();  // the tile's reads
+          asm volatile("" ::: "memory");
+          issue(tn, 0);
+        }
         t = tn, cl = cn, ++n;
       };
       while (t >= 0) {
@@ -774,15 +782,11 @@ __global__ __launch_bounds__(256, DH == 64 ? 3 : 2) void attn_scored_kernel(Attn
   scored_item<DH, 4, false, CAP, BIAS>(a, smem, b, kvh, g, qb, 0);
 }
 
-// Few queries: blocks of 32, the waves (four, or two at head_dim 128, whose
-// rings fill the LDS) and the splits (grid y) divide the keys.
-template <int DH>
-constexpr int ks_waves() {
-  return DH == 64 ? 4 : 2;
-}
+// Few queries: blocks of 32, the four waves and the splits (grid y) divide the keys.
+constexpr int kKsWaves = 4;
 template <int DH, int CAP, bool BIAS>
-__global__ __launch_bounds__(64 * ks_waves<DH>()) void attn_scored_few_kernel(AttnScoredArgs a) {
-  constexpr int NW = ks_waves<DH>();
+__global__ __launch_bounds__(64 * kKsWaves) void attn_scored_few_kernel(AttnScoredArgs a) {
+  constexpr int NW = kKsWaves;
   __shared__ __attribute__((aligned(16))) char smem[lds_bytes<DH, NW, true>()];
   const int G = a.pack ? 1 : a.H / a.Hkv;
   const int qb = blockIdx.x % a.n_blocks, r = blockIdx.x / a.n_blocks;
@@ -884,8 +888,7 @@ Plan plan_of(const AttnScoredArgs& a) {
   p.pack = G > 1 && static_cast<int64_t>(a.max_q) * G <= 32;
   p.n_blocks = p.pack ? 1 : (a.max_q + 31) / 32;
   p.items = (p.pack ? static_cast<int64_t>(a.B) * a.Hkv : heads) * p.n_blocks;
-  const int nw = a.Dh == 64 ? 4 : 2;
-  p.splits = static_cast<int>(std::clamp<int64_t>(kCus / std::max<int64_t>(1, p.items), 1, std::max<int64_t>(1, tiles / (2 * nw))));
+  p.splits = static_cast<int>(std::clamp<int64_t>(kCus / std::max<int64_t>(1, p.items), 1, std::max<int64_t>(1, tiles / kKsWaves)));
   return p;
 }
 
@@ -893,7 +896,7 @@ template <int DH, int CAP, bool BIAS>
 void launch_mfma(const AttnScoredArgs& a, const Plan& p, hipStream_t st) {
   if (p.few) {
     attn_scored_few_kernel<DH, CAP, BIAS>
-        <<<dim3(static_cast<unsigned>(p.items), static_cast<unsigned>(p.splits)), 64 * ks_waves<DH>(), 0, st>>>(a);
+        <<<dim3(static_cast<unsigned>(p.items), static_cast<unsigned>(p.splits)), 64 * kKsWaves, 0, st>>>(a);
     return;
   }
   const int64_t pairs = static_cast<int64_t>(a.B) * a.Hkv, pairs8 = (pairs + 7) / 8 * 8;
