@@ -311,9 +311,8 @@ int sjh_add_ln(float* X, const void* R, const float* W, const float* B, void* Y,
  * population variance) or the RMS norm (v / sqrt(mean(v^2) + eps) * w + b).
  * sjh_add_ln is post = nothing, pre = LayerNorm, without gate or scales.  No
  * counterpart in the reference, whose blocks have no norm after them.
- * D up to 8192.  Row strides are in elements, 0 standing for D; rows whose
- * strides and addresses allow 16-byte accesses (8-byte for bf16) of four
- * values are the fast ones.  x_out may be x, and y may be r, with the same
+ * D up to 8192.  Row strides are in elements, 0 standing for D; any alignment of
+ * the types is as fast as another.  x_out may be x, and y may be r, with the same
  * strides; no other outputs and inputs may overlap.  Sums are taken in double.
  * A NaN in r or x, or an infinity under LayerNorm, reaches its own row only. */
 enum { SJH_NORM_NONE = 0, SJH_NORM_LAYER = 1, SJH_NORM_RMS = 2 };
