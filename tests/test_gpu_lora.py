@@ -127,6 +127,18 @@ def test_lora(M, N, K, R, n, dtype):
 
 
 # shapes of the fp32-product kernel: K no multiple of 64, rows no vector load takes, bf16 among them
+# the first product's blocks of 64 rows: one piece of K, fewer and more than its
+# ring holds; a rank block, two and four, a second sweep; blocks of one adapter, of
+# none, of many, and where requests meet
+@pytest.mark.parametrize("dtype", ["bf16", "fp8"])
+@pytest.mark.parametrize("M,N,K,R,n,rows", [(8192, 64, 64, 16, 70, 1), (8200, 40, 192, 24, 5, 100), (8255, 96, 320, 65, 3, 64), (9001, 36, 768, 130, 2, 5000)])
+def test_lora_many_rows(M, N, K, R, n, rows, dtype):
+    print(f"lora many {M}x{N}x{K} R={R} n={n} {rows} {dtype}", flush=True)
+    c = Case(M, N, K, R, n, mixed(M, n) if rows == 1 else runs(M, n, rows), dtype=dtype)
+    c.run()
+    c.check()
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("M,N,K,R,n,off,pad", [(5, 3, 1, 1, 1, 0, 0), (33, 70, 51, 7, 3, 0, 0), (200, 130, 128, 16, 4, 1, 1), (700, 600, 100, 33, 5, 0, 3), (1, 9, 64, 4, 2, 1, 0)])
 def test_lora_any_shape(M, N, K, R, n, off, pad, dtype):
