@@ -311,8 +311,8 @@ int sjh_add_ln(float* X, const void* R, const float* W, const float* B, void* Y,
  * population variance) or the RMS norm (v / sqrt(mean(v^2) + eps) * w + b).
  * sjh_add_ln is post = nothing, pre = LayerNorm, without gate or scales.  No
  * counterpart in the reference, whose blocks have no norm after them.
- * D up to 8192.  Row strides are in elements, 0 standing for D; any alignment of
- * the types is as fast as another.  x_out may be x, and y may be r, with the same
+ * D up to 8192.  Row strides are in elements, 0 standing for D; rows at any
+ * alignment of their type take the same accesses.  x_out may be x, and y may be r, with the same
  * strides; no other outputs and inputs may overlap.  Sums are taken in double.
  * A NaN in r or x, or an infinity under LayerNorm, reaches its own row only. */
 enum { SJH_NORM_NONE = 0, SJH_NORM_LAYER = 1, SJH_NORM_RMS = 2 };
@@ -366,7 +366,7 @@ int sjh_attn_log2(const void* qkv, const int32_t* lens, void* O, int32_t B, int3
  * are padding and a window (src/tensor.cpp:186-192).
  *
  * Sequence b's queries are rows q_start[b] + [0, q_len[b]) of q and o, its keys
- * rows k_start[b] + [0, k_len[b]) of k and v; head h of row t is at
+ * rows k_start[b] + [0, k_len[b]) of k and v (keys may be shared, query rows not); head h of row t is at
  * q + t ld_q + h Dh (k, v: head h / (H / Hkv)).  Rows of o outside every
  * sequence are left as they were.  Starts and lengths are clamped to q_rows,
  * k_rows, max_q and max_k (so max_q and max_k must bound the lengths), q_pos to

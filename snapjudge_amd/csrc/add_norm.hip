@@ -158,8 +158,7 @@ __global__ __launch_bounds__(64 * WPB) void add_norm_kernel(AddNormArgs a) {
     gate = a.gate + static_cast<int64_t>(id) * D;
   }
   const float* xr = a.x + row * a.ld_x;
-  // (read before x_out, which may be x, is written)
-  const float first_x = WAVES == 1 ? 0.f : xr[0];
+  float first_x = WAVES == 1 ? 0.f : xr[0];
   const T* rr = a.r ? static_cast<const T*>(a.r) + row * a.ld_r : nullptr;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -192,6 +191,11 @@ __global__ __launch_bounds__(64 * WPB) void add_norm_kernel(AddNormArgs a) {
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int k = 0; k < 4; ++k) x[i][k] *= a.x_scale;
+  }
+  if constexpr (WAVES > 1) {
+    // x_out may be x: every wave has read x[0] before any wave writes it
+    asm volatile("" : "+v"(first_x));
+    __syncthreads();
   }
   if (a.x_out) {
     float* xo = a.x_out + row * a.ld_xo;

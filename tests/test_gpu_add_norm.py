@@ -161,3 +161,21 @@ def test_add_norm_in_a_graph_and_on_a_stream():
         call(**kw)
         torch.cuda.synchronize()
         assert torch.equal(got[0], xo) and torch.equal(got[1], y), i
+
+
+@pytest.mark.parametrize("post,pre", [("none", "ln"), ("rms", "ln"), ("ln", "rms")])
+@pytest.mark.parametrize("M,D", [(700, 260), (900, 1023), (2000, 1028), (1500, 2049), (800, 8190)])
+def test_add_norm_in_place(M, D, post, pre):
+    """x_out = x and y = r give the bits of outputs of their own."""
+    print(f"add_norm in place {M}x{D} {post} {pre}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(D)
+    x, r = (torch.randn(M, D, generator=g, device="cuda") + 3 for _ in range(2))
+    kw = dict(x_scale=1.5, r_scale=2.0, eps=1e-5, post_norm=KIND[post], pre_norm=KIND[pre], M=M, D=D, dtype=sj.SJH_F32)
+    xo, y = torch.empty_like(x), torch.empty_like(r)
+    call(x=x, r=r, x_out=xo, y=y, **kw)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        x1, r1 = x.clone(), r.clone()
+        call(x=x1, r=r1, x_out=x1, y=r1, **kw)
+        torch.cuda.synchronize()
+        assert torch.equal(x1, xo) and torch.equal(r1, y)
