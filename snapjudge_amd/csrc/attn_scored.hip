@@ -13,7 +13,7 @@
 // query), the scores' cap, bias, masks and exponentials in registers, O^T += V^T
 // P^T with P^T straight from the accumulator (its key order is the MFMA's k
 // order) and V^T through transposed LDS reads.  K and V tiles come by
-// direct-to-LDS loads into a two-stage ring, XOR-swizzled.
+// direct-to-LDS loads into a ring, XOR-swizzled.
 //
 // Which tiles: the mask's positions and each tile's range of documents decide
 // before anything of the tile is read (TileIter); a tile that every query of
@@ -126,8 +126,8 @@ template <int DH, int NW, bool KS, int CAPM, bool BIAS>
 __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem, int b, int kvh, int g, int qb, int split) {
   constexpr bool CAP = CAPM != CAP_NONE;
   // Capped scores without a bias lie within [-cap, cap]: with the cap at most
-  // kFixedCap in log2, weights 2^s need no running maximum (8192 of them and
-  // their products stay far inside fp32 and bf16).
+  // kFixedCap in log2, weights 2^s need no running maximum: sums of 2^29 of them
+  // fit fp32, and rows whose sums or outputs come near its ends run again.
   constexpr bool FIXED = CAPM == CAP_FIXED;
   static_assert(!FIXED || !BIAS, "a bias leaves no lower bound");
   constexpr int ROWB = DH * 2, TILEB = kTile * ROWB;          // bytes of a row, of a K or V tile
@@ -262,7 +262,7 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
   const float cap2 = uni(CAP ? a.softcap * kLog2e : 0.f);    // the cap in log2
   const float ucap = CAP ? a.scale / a.softcap : 0.f;        // u = ucap raw
   // y = raw (A0 + w (A1 + w (A2 + w A3))), w = raw^2
-  const float B0 = cap2 * ucap, B1 = B0 * ucap * ucap, B2 = B1 * ucap * ucap, B3 = B2 * ucap * ucap;
+  const float B0 = c, B1 = B0 * ucap * ucap, B2 = B1 * ucap * ucap, B3 = B2 * ucap * ucap;
   const float A0 = uni(B0 * kTanh0), A1 = uni(B1 * kTanh1), A2 = uni(B2 * kTanh2), A3 = uni(B3 * kTanh3);
   const float raw_max = uni(CAP && fabsf(A3) < INFINITY ? kTanhMax / ucap : -1.f);
   const float kexp = uni(2.f * kLog2e * ucap);
@@ -293,7 +293,7 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
   float m_i, l_i, l_j;
 
   // One tile from ring slot `slot`.  PART: masks.  MAXR: the running maximum; else
-  // weights are 2^s as they come (pass_check).  NF: V through v_map(mode) where
+  // weights are 2^s as they come (checked after the pass).  NF: V through v_map(mode) where
   // mode >= 0.  side (whole tiles under a linear bias): 1 keys before the queries,
   // 3 after.
   auto tile = [&](auto part_tag, auto max_tag, auto nf_tag, int mode, int slot, int tl, int side) {
@@ -354,7 +354,9 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
 #pragma unroll
         for (int e = 0; e < 16; ++e) tmax = fmaxf(tmax, sc[jb][e]);
       tmax = wave_max32(tmax);
-      tmax = CAP ? cap_exact(tmax) : __builtin_fmaf(tmax, c, tb);  // both rise with the score
+      // (all rise with the score; the form that the tile's scores take, whose errors
+      // a large cap would otherwise set apart)
+      tmax = !CAP ? __builtin_fmaf(tmax, c, tb) : small ? tmax * cap_poly(tmax) : cap_exact(tmax);
     } else {
       const int4 qi4 = *qinfo;
       const float d0 = static_cast<float>(qi4.x - base);
@@ -567,6 +569,7 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
         else
           wait_vmcnt<(NS - 2) * 2 * NL>();
         __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");  // (the barrier alone orders no reads for the compiler)
         const int last = slot == 0 ? NS - 1 : slot - 1;  // the slot that the tile before was in
         if (tq[NS - 1] >= 0) issue(tq[NS - 1], last);
         if (cq[0] != 0) run(cq[0], whole_tag, redo_tag, mode, slot, tq[0]);
@@ -630,13 +633,14 @@ __device__ __forceinline__ void scored_item(const AttnScoredArgs& a, char* smem,
     return bad;
   };
   {
-    // Without the maximum (pass_check): every row's weight sum must lie in [2^-60,
-    // 2^64].  Then nothing overflowed, and a weight that flushed to zero (below
-    // 2^-126) is under 2^-50 of the largest.  Else (a row that sees no key
-    // among them, but for scores that a cap bounds) the workgroup runs again with
-    // the maximum, as it does for an output that is not finite.
+    // Without the maximum: every row's weight sum must lie in [2^-60, 2^64].  Then
+    // nothing overflowed, and what flushed to zero (weights, and their products
+    // with values, below 2^-126) is under 2^-66 per key of the sum.  Else (a row
+    // that sees no key among them, but where a cap keeps the sums of others above
+    // 0) the workgroup runs again with the maximum, as it does for an output that is
+    // not finite.
     bool again = unclean();
-    if constexpr (!KS && !FIXED) again |= !(l_i >= 0x1p-60f && l_i <= 0x1p64f);
+    if constexpr (!KS) again |= FIXED ? l_i > 0.f && l_i < 0x1p-60f : !(l_i >= 0x1p-60f && l_i <= 0x1p64f);
     if (vote(again)) {  // uniform over the workgroup
       pass(std::true_type{}, -1);
       again = vote(unclean());

@@ -362,3 +362,43 @@ def test_attn_scored_in_graphs_on_streams_and_twice_at_once():
             sj.check(sj.lib().sjh_attn_scored(C.byref(a), C.c_void_p(s.cuda_stream)))
         torch.cuda.synchronize()
         assert all(torch.equal(c.o, w) for c, w in zip(cs, want))
+
+
+@pytest.mark.parametrize("Dh,q,B", [(64, 100, 4), (128, 100, 4), (64, 3, 1)])
+def test_attn_scored_small_values_under_low_scores(Dh, q, B):
+    """Every score at the cap's lower end (weights 2^-95 of 1), values of 1e-12: their
+    products are below fp32's range without a maximum."""
+    print(f"attn_scored small values {Dh} {q}", flush=True)
+    c = Case([q] * B, [q] * B, H=64, Dh=Dh, cap=66.0)
+    c.q.fill_(9.0)
+    c.k.fill_(-9.0)
+    c.v *= 1e-12
+    c.run()
+    c.check(seqs=[B - 1])
+    assert float(c.o[:q].abs().max()) > 0
+
+
+@pytest.mark.parametrize("H,q", [(2, 3), (64, 130)])
+@pytest.mark.parametrize("cap", [1e9, 1e10, 1e37])
+def test_attn_scored_caps_far_above_the_scores(cap, H, q):
+    """cap tanh(s / cap) = s to 2^-40 here.  A score is off by 1e-5 of its size (the
+    polynomial's factor of it, 9e-6, and fp32's roundings), a weight by twice the
+    largest score's and bf16's 2^-8, as in the bound above."""
+    print(f"attn_scored cap {cap} {H} {q}", flush=True)
+    c = Case([q] * 4, [300] * 4, H=H, cap=cap, amp=60.0)
+    c.run()
+    got = c.o.double().cpu().numpy()
+    q_, k, v = (t.double().cpu().numpy() for t in (c.q, c.k, c.v))
+    for b in (0, 3):
+        for h in (0, H - 1):
+            s = q_[c.qs[b]:c.qs[b] + q, h] @ k[c.ks[b]:c.ks[b] + 300, h].T / 8
+            assert np.abs(s).max() > 100  # (144 in log2: past fp32 without a maximum)
+            w = np.exp(s - s.max(1, keepdims=True))
+            w /= w.sum(1, keepdims=True)
+            vv = v[c.ks[b]:c.ks[b] + 300, h]
+            want = w @ vv
+            d = 2 * 1e-5 * np.abs(s).max(1, keepdims=True) + 16 * U + 2.0 ** -8
+            lim = 1.05 * d * np.einsum("ij,ijd->id", w, np.abs(vv[None] - want[:, None])) + 2 * 308 * U * (w @ np.abs(vv))
+            lim = lim + 2.0 ** -8 * (np.abs(want) + lim)
+            err = np.abs(got[c.qs[b]:c.qs[b] + q, h] - want)
+            assert np.all(err <= lim), (b, h, float((err / lim).max()))
