@@ -1047,8 +1047,9 @@ struct DTile {
 template <typename OutT>
 __device__ void splitk_output(const GemmArgs& g, int S, int m, int n);
 
-// One WM x WN block of an adapter product by a wave, operands straight from memory in the K order of the staged kernels (the same bits), the adapters
-// by lora_acc: what EPI_LORAK does with a tile that met values that are not finite.
+// One WM x WN block of an adapter product by a wave, operands straight from memory
+// in the K order of the staged kernels (the same bits), the adapters by lora_acc:
+// what EPI_LORAK does with a tile that met values that are not finite.
 template <int BM, int BN, int WM, int WN, int TI, int TJ, int EPI, typename OutT>
 __device__ __forceinline__ void lora_redo(const GemmArgs& g, int m0, int tile_n, int wm, int wn, int l32, int hb) {
   f32x16_t acc[TI][TJ];
@@ -1303,16 +1304,16 @@ __global__ __launch_bounds__(64 * WGM * WGN, EPI == EPI_LORAK ? (WGM * WGN >= 16
       if (kt + NS - 1 < nt) issue_x(kt + NS - 1 - nk, (kt + NS - 1) % NS);
       if (kt >= nk) {  // 0 times a B value that is not finite is NaN
         const char* sb = dsmem + (kt % NS) * TT::STAGE_BYTES;
-                typedef __attribute__((ext_vector_type(2))) __bf16 bf2_t;
-                const bf2_t zero = {};
+        typedef __attribute__((ext_vector_type(2))) __bf16 bf2_t;
+        const bf2_t zero = {};
 #pragma unroll
-                for (int s = 0; s < KS; ++s)
+        for (int s = 0; s < KS; ++s)
 #pragma unroll
-                  for (int j = 0; j < TJ; ++j) {
-                    const bf16x8_t w = *reinterpret_cast<const bf16x8_t*>(sb + w_row0 + j * 32 * RB + ((2 * s + hb) ^ xr) * 16);
+          for (int j = 0; j < TJ; ++j) {
+            const bf16x8_t w = *reinterpret_cast<const bf16x8_t*>(sb + w_row0 + j * 32 * RB + ((2 * s + hb) ^ xr) * 16);
 #pragma unroll
-                    for (int t = 0; t < 8; t += 2) nonfin = __builtin_amdgcn_fdot2_f32_bf16((bf2_t){w[t], w[t + 1]}, zero, nonfin, false);
-                  }
+            for (int t = 0; t < 8; t += 2) nonfin = __builtin_amdgcn_fdot2_f32_bf16((bf2_t){w[t], w[t + 1]}, zero, nonfin, false);
+          }
       }
       compute(kt);
     }
@@ -2217,8 +2218,15 @@ Tile pick_tile(const GemmArgs& g) {
   if (count_tiles(g, 128, 64) <= cus) return T128x64;
   const int64_t t128 = count_tiles(g, 128, 128);
   if (t128 <= cus) return T128D;
-  if (g.epi == EPI_LORA) return T128;
-  if (g.epi == EPI_LORAK) return t128 <= 2 * cus ? T128 : TPERS;
+  if (g.epi == EPI_LORA) return T128;  // (the 256 x 256 kernels have no registers for lora_acc)
+  if (g.epi == EPI_LORAK) {
+    // 256 x 256 tiles where their last round over the CUs leaves no more than a
+    // quarter of them idle: N 2304, K 768, rank 64, 8192 rows (1.1 rounds) 50.0 us in
+    // 128 x 128 tiles, 63.0 in 256 x 256; 12000 rows, rank 32 (1.7) 67.4, 65.9; 18432,
+    // rank 16 (2.5) 100.1, 96.0
+    const int64_t t256 = count_tiles(g, 256, 256), slots = (t256 + cus - 1) / cus * cus;
+    return 4 * t256 >= 3 * slots ? TPERS : T128;
+  }
   const int short_k = g.w_dtype == DT_FP8 ? 1024 : g.epi == EPI_STORE ? 512 : 256;
   if (t128 <= 2 * cus || (g.K <= short_k && 8 * count_tiles(g, 256, 256) < 5 * cus) || !pers_ok(g)) return T128;
   return TPERS;
