@@ -767,8 +767,9 @@ __global__ __launch_bounds__(256, DH == 64 ? 3 : 2) void attn_scored_kernel(Attn
   const int G = a.H / a.Hkv, per = G * a.n_blocks;
   int pair, r;
   if (a.pack < 0) {
-    pair = blockIdx.x / per;
-    r = blockIdx.x - pair * per;
+    const int np = a.B * a.Hkv;  // causal: the longest rows of all pairs first
+    pair = a.causal ? blockIdx.x % np : blockIdx.x / per;
+    r = a.causal ? blockIdx.x / np : blockIdx.x - pair * per;
   } else if (a.causal) {  // the longest rows of all of the XCD's pairs first
     const int xcd = blockIdx.x & 7, kx = blockIdx.x >> 3, np = (a.B * a.Hkv + 7) / 8;
     r = kx / np;
@@ -880,8 +881,18 @@ Plan plan_of(const AttnScoredArgs& a) {
     p.splits = static_cast<int>(std::clamp<int64_t>(kCus / std::max<int64_t>(1, p.items), 1, std::max<int64_t>(1, tiles / 2)));
     return p;
   }
-  const int64_t full = heads * ((a.max_q + 127) / 128);
-  if (full >= kCus) {
+  // Blocks of 128 queries, or of 32 whose keys the waves and splits divide.  A CU
+  // takes one of the latter at a time, 5.5 us + 0.4 us a tile (head_dim 64, cap), and
+  // 64 CUs of them are the work of 64 blocks of 128; those run side by side, 4 us +
+  // 1.6 us a tile while there are no more than CUs.  Measured (12 heads, 512-key
+  // sequences of 512 queries; 8, 16, 20 blocks of 128 a head): 18.6, 27.7, 34.9 us in
+  // 32s, 16.4, 16.9, 18.2 in 128s; (8192 keys; 8 and 16 blocks) 112, 168 in 32s, 201,
+  // 206 in 128s.  Where a block of 32 holds the queries of all heads of a key head,
+  // keys are read once for them: 64 single tokens of 32 heads on 8 key heads over
+  // 2048 keys 60.9 us, 186 in 128s.
+  p.pack = G > 1 && static_cast<int64_t>(a.max_q) * G <= 32;
+  const int64_t full = heads * ((a.max_q + 127) / 128), rounds = (full + kCus / 4 - 1) / (kCus / 4);
+  if (!p.pack && rounds > 1 && rounds * (14 + tiles) >= 10 + 4 * tiles) {
     p.rows = 128;
     p.n_blocks = (a.max_q + 127) / 128;
     p.items = full;
@@ -889,7 +900,6 @@ Plan plan_of(const AttnScoredArgs& a) {
   }
   p.few = true;
   p.rows = 32;
-  p.pack = G > 1 && static_cast<int64_t>(a.max_q) * G <= 32;
   p.n_blocks = p.pack ? 1 : (a.max_q + 31) / 32;
   p.items = (p.pack ? static_cast<int64_t>(a.B) * a.Hkv : heads) * p.n_blocks;
   p.splits = static_cast<int>(std::clamp<int64_t>(kCus / std::max<int64_t>(1, p.items), 1, std::max<int64_t>(1, tiles / kKsWaves)));
@@ -906,7 +916,10 @@ void launch_mfma(const AttnScoredArgs& a, const Plan& p, hipStream_t st) {
   const int64_t pairs = static_cast<int64_t>(a.B) * a.Hkv, pairs8 = (pairs + 7) / 8 * 8;
   AttnScoredArgs b = a;
   int64_t wgs = p.items;
-  if (4 * pairs >= 3 * pairs8)
+  // Pairs of sequence and key head to an XCD each where that fills 7/8 of them (8192
+  // keys, not causal; 3 pairs of 4 heads: 762 us so, 337 in plain order; 10 of one: 428,
+  // 319; 12: 438, 332; 192 pairs, 512 keys: 30.2, 32.9)
+  if (8 * pairs >= 7 * pairs8)
     wgs = pairs8 * (a.H / a.Hkv) * p.n_blocks;
   else
     b.pack = -1;
