@@ -19,11 +19,21 @@
 // before anything of the tile is read (TileIter); a tile that every query of
 // a wave sees whole runs without masks.  Two shapes:
 //  - four waves of 32 queries share the ring (128 queries a workgroup; three
-//    workgroups share a CU at head_dim 64, two at 128);
+//    workgroups share a CU at head_dim 64, two at 128), without a running maximum
+//    at first: rows whose weight sum or outputs come out of range run again;
 //  - few queries: a workgroup owns 32 (with shared key heads, the queries of
 //    all heads of the group where they fit), each wave takes every NW-th
 //    needed tile through a ring of its own, further workgroups further tiles
 //    (splits); sums meet in LDS and, split, in a second launch.
+//
+// What bounds it: the vector pipe.  A lane's score costs the cap's polynomial (five
+// instructions), the exponential (a quarter of the rate), its rounding and its
+// share of the sum, about 50 cycles per 64 scores against 16 of the matrix pipe at
+// head_dim 64; few queries over long keys are bound by the bytes of K and V.
+// Measured, bf16: 16 sequences of 1800 to 2048 tokens of packed documents, 12 heads
+// of 64, cap, 156 us; two causal ones of 5000 and 8192 with distance biases 196 us; 3
+// sequences of 6000 to 8191 keys, a few queries each, 16 heads of 128 on 4 key
+// heads, 17 us and 5 for the join.
 //
 // A masked key takes no part, whatever its values: its score is replaced, and
 // where an infinite or NaN V row met a weight of 0 (the output is then not
