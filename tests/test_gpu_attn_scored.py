@@ -402,3 +402,28 @@ def test_attn_scored_caps_far_above_the_scores(cap, H, q):
             lim = lim + 2.0 ** -8 * (np.abs(want) + lim)
             err = np.abs(got[c.qs[b]:c.qs[b] + q, h] - want)
             assert np.all(err <= lim), (b, h, float((err / lim).max()))
+
+
+@pytest.mark.parametrize("Dh,H,Hkv", [(64, 8, 2), (128, 8, 2), (64, 32, 1)])
+def test_attn_scored_many_sequences_of_few_tokens(Dh, H, Hkv):
+    """More sequences than CUs, the queries of a key head's heads in one block of 32."""
+    print(f"attn_scored many few {Dh} {H} {Hkv}", flush=True)
+    ql, kl = ([1, 2, 0, 4], [1, 64, 3, 130]) if H == 8 else ([1, 1, 0, 1], [700, 64, 3, 65])
+    c = Case(ql * 80, kl * 80, H=H, Hkv=Hkv, Dh=Dh, cap=20.0, causal=True, prefix=[0, 5, 1, 40] * 80, docs=lambda b, j: j // 33)
+    c.run()
+    c.check(seqs=[0, 1, 2, 3, 158, 159, 318, 319])
+
+
+@pytest.mark.parametrize("B,H,Hkv", [(3, 9, 9), (3, 9, 3), (1, 30, 30), (5, 12, 3)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attn_scored_orders_of_blocks(B, H, Hkv, causal):
+    """Pairs of sequence and key head that fill the XCDs' turns and that do not; every
+    block of every head is written (the rows of one are told apart by their values)."""
+    print(f"attn_scored orders {B} {H} {Hkv} {causal}", flush=True)
+    L = [1300 - 7 * b for b in range(B)]
+    c = Case(L, L, H=H, Hkv=Hkv, causal=causal, cap=30.0, window=200)
+    c.run()
+    for b in range(B):
+        assert not bool((c.o[c.qs[b]:c.qs[b] + L[b]] == 7).all(-1).any()), b
+    for rows in ((0, 40), (630, 650), (1260, 1300)):
+        c.check(seqs=[0, B - 1], rows=rows)
