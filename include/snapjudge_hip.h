@@ -360,10 +360,10 @@ int sjh_attn_log2(const void* qkv, const int32_t* lens, void* O, int32_t B, int3
  *   j < prefix, or
  *   (not causal, or j <= p) and (window 0, or |p - j| <= window) and
  *   (no documents, or q_doc of the query's row == k_doc of the key's row).
- * A query that sees no key, or whose scores are all -infinity, gives zeros.  A key takes part only where it is
- * visible, whatever its values (infinities and NaN among them).  sjh_attn is
- * the padded, unmodified case; no counterpart in the reference, whose masks
- * are padding and a window (src/tensor.cpp:186-192).
+ * A query that sees no key, or whose scores are all -infinity, gives zeros.  A
+ * key takes part only where it is visible, whatever its values (infinities and
+ * NaN among them).  sjh_attn is the padded, unmodified case; no counterpart in
+ * the reference, whose masks are padding and a window (src/tensor.cpp:186-192).
  *
  * Sequence b's queries are rows q_start[b] + [0, q_len[b]) of q and o, its keys
  * rows k_start[b] + [0, k_len[b]) of k and v (keys may be shared, query rows not); head h of row t is at
